@@ -277,6 +277,96 @@ int rbt_hip_model_create(rbt_hip *h, const rbt_config *cfg, void **model_dev);
  * "q_norm", "k_norm", "ffn_norm", "router", "experts" of layer `layer`. */
 int rbt_hip_tensor(rbt_hip *h, const char *name, int layer, uint64_t *offset, uint64_t *bytes);
 
+/* ---- a paged key/value cache (no counterpart in the reference, whose State holds one sequence of a fixed
+ * context): requests of any lengths share one pool of blocks ("pages") of block_size positions each. A step
+ * runs rbt_hip_paged_plan_dev once, then per layer rbt_hip_paged_append_dev and rbt_hip_paged_attn_dev. All
+ * take device pointers, are asynchronous on the handle stream and can be captured into a graph (after
+ * rbt_hip_paged_reserve): every length is read on the device, so a captured step replays for other lengths. ---- */
+
+/* One layer's cache: block b's keys are k + b * block_stride, [n_kv_heads][block_size][head_dim] elements of
+ * dtype (RBT_DT_F32 or RBT_DT_BF16), its values v + b * block_stride alike. block_stride 0: blocks follow each
+ * other. head_dim 1..256, n_blocks * block_size below 2^31. */
+typedef struct {
+    int32_t n_blocks, block_size, n_kv_heads, head_dim, dtype;
+    void *k, *v;
+    uint64_t block_stride; /* elements */
+} rbt_paged_kv;
+
+/* The requests of a step: request r has kv_len[r] positions in the cache, this step's among them; position p
+ * is row p % block_size of block tables[r * max_blocks + p / block_size]. Rows q_start[r] .. q_start[r + 1] - 1
+ * of the step's row buffers are its new tokens, the last positions of the request. n_req up to 4096. A request
+ * without new rows takes no part. */
+typedef struct {
+    int32_t n_req, max_blocks;
+    const int32_t *tables;  /* [n_req][max_blocks] */
+    const int32_t *kv_len;  /* [n_req] */
+    const int32_t *q_start; /* [n_req + 1], ascending from 0 */
+} rbt_paged_batch;
+
+/* What a step's plan reads and writes (device arrays). Request r has len[r] positions and gets new_len[r] more,
+ * or ends where new_len[r] is negative (its blocks go back to the free list). free_list is a stack of the
+ * *n_free blocks that no request holds. kv_len may be len, and n_free_out n_free; else no two arrays overlap. */
+typedef struct {
+    int32_t n_req, max_blocks, n_blocks, block_size;
+    int32_t max_tokens;     /* rows of the step's buffers: slots and positions are filled up to it */
+    const int32_t *len;     /* [n_req] */
+    const int32_t *new_len; /* [n_req] */
+    int32_t *tables;        /* [n_req][max_blocks]: the blocks of the new positions are filled in */
+    int32_t *free_list;     /* [n_blocks] */
+    const int32_t *n_free;  /* [1] */
+    int32_t *kv_len;        /* [n_req] out: len + new_len; 0 for a request that ended */
+    int32_t *n_free_out;    /* [1] out */
+    int32_t *q_start;       /* [n_req + 1] out: each request's first row */
+    int32_t *slots;         /* [max_tokens] out: block * block_size + row of each new token, -1 behind the last */
+    int32_t *positions;     /* [max_tokens] out: each new token's position, -1 behind the last */
+    int32_t *status;        /* [1] out */
+} rbt_paged_plan;
+
+/* The rows of a step's new tokens. Strides are in floats from row to row, 0: the rows follow each other. */
+typedef struct {
+    int32_t n_tokens, n_heads;
+    const float *q, *k, *v; /* [n_tokens] rows of n_heads * head_dim, n_kv_heads * head_dim (k, v); q may be NULL */
+    uint64_t q_stride, k_stride, v_stride;
+    float *q_out;                 /* [n_tokens][n_heads * head_dim], contiguous; may be q where q is contiguous */
+    const float *q_norm, *k_norm; /* QK-norm weights over the whole rows (rabbit2.c:475-478); NULL: none */
+    float eps;
+    const float *rope;        /* [n_rope][head_dim / 2][2]: (cos, sin) of each position's angles; NULL: none */
+    int32_t n_rope;
+    const int32_t *positions; /* [n_tokens]; read for rope only */
+    const int32_t *slots;     /* [n_tokens] */
+} rbt_paged_rows;
+
+/* Block tables, slot map and row starts of a step from the requests' lengths. Blocks of ended requests are
+ * pushed onto the free stack in (request, page) order, then the blocks that new positions need are popped
+ * from its top in the same order; blocks already in a row stay. *status: 0; the number of blocks lacking; or -1
+ * where an argument array is out of range (len or len + new_len outside [0, max_blocks * block_size], more new
+ * tokens than max_tokens, a free count outside [0, n_blocks], also after the pushes). With a status other than 0
+ * nothing is granted: kv_len = len, q_start all 0, slots and positions all -1 (so that the calls below leave
+ * everything as it is), free list and tables unchanged. */
+int rbt_hip_paged_plan_dev(rbt_hip *h, const rbt_paged_plan *plan);
+
+/* QK-norm and RoPE (the engine's, rabbit2.c:410-423, :475-480: pairs i and i + head_dim / 2) of the new rows: q
+ * to q_out, k and v into the cache at their slots, rounded to the cache's type (to nearest even). A token
+ * whose slot is outside the cache, or whose position is outside the table with rope, is passed over: nothing of
+ * it is written. No two tokens have one slot. */
+int rbt_hip_paged_append_dev(rbt_hip *h, const rbt_paged_kv *kv, const rbt_paged_rows *rows);
+
+/* Causal attention of the new rows over their requests' cached positions (their own among them):
+ * out[t][h] = sum_j softmax_j(scale * q[t][h] . k_j) v_j over the positions j of the request up to the row's own
+ * p, with window > 0 over p - window + 1 .. p only. Query head h reads key/value head h / (n_heads /
+ * n_kv_heads). q and out hold T rows of n_heads * head_dim floats, q_stride / out_stride floats apart (0: they
+ * follow each other); scale 0: 1 / sqrt(head_dim). Sums and the softmax run in f32; the q rows enter the
+ * products exactly, the weights with at least 16 bits. A position outside the table's length or on a block
+ * outside [0, n_blocks) is not seen; a row that sees none is 0; rows of no request (behind the last one's)
+ * are left as they are. What lies behind a row's own position, infinities and NaN too, does not reach it. */
+int rbt_hip_paged_attn_dev(rbt_hip *h, const rbt_paged_kv *kv, const rbt_paged_batch *batch, const float *q,
+                           uint64_t q_stride, int T, int n_heads, float scale, int window, float *out,
+                           uint64_t out_stride);
+
+/* Allocates the attention's workspace (64 MiB, of one size for every call and held until rbt_hip_free), which the
+ * first call does otherwise; needed before capturing one. */
+int rbt_hip_paged_reserve(rbt_hip *h);
+
 /* ---- device memory and stream plumbing for hosts without their own HIP code ---- */
 int rbt_hip_malloc(rbt_hip *h, void **dev, uint64_t bytes);
 int rbt_hip_free_dev(rbt_hip *h, void *dev);
@@ -293,7 +383,7 @@ void *rbt_hip_stream(rbt_hip *h); /* the hipStream_t all of this handle's work r
  * lists -- and "combine", and its "down_combine" is the down GEMM alone); rbt_hip_forward adds
  * "embed", "attn_norm", "qkv" (RMSNorm + q/k/v), "attention", "attn_merge", "wo", "ffn_norm",
  * "lm_head" (final norm + lm_head, with the argmax inside where the rows allow) and "argmax"
- * (otherwise). Batched steps launch fewer: from 512 (sequence, head) pairs the attention writes its
+ * (otherwise); the paged cache's calls "paged_plan", "paged_append", "paged_attn" and "paged_merge". Batched steps launch fewer: from 512 (sequence, head) pairs the attention writes its
  * output without "attn_merge", and on the grouped path "combine" also runs the RMSNorm that the
  * next step would time as "attn_norm". rbt_hip_generate is never timed this way. Modes (on):
  *   0  off.

@@ -17,6 +17,7 @@
 #include <sys/stat.h>
 #include <unistd.h>
 
+#include "paged.h"
 #include "rbt2_internal.h"
 
 using namespace rbt;
@@ -51,11 +52,13 @@ enum ProfKernel {
     kProfRouter, kProfTopk, kProfGateup, kProfDown, kProfDispatch, kProfCombine,
     // the rest of the forward pass (rbt_hip_forward with profiling on)
     kProfEmbed, kProfAttnNorm, kProfQkv, kProfAttn, kProfAttnMerge, kProfWo, kProfFfnNorm, kProfLmHead, kProfArgmax,
+    kProfPagedPlan, kProfPagedAppend, kProfPagedAttn, kProfPagedMerge,
     kProfCount
 };
 const char *const kProfNames[kProfCount] = {"router", "topk", "gateup", "down_combine", "dispatch", "combine",
                                             "embed", "attn_norm", "qkv", "attention", "attn_merge", "wo", "ffn_norm",
-                                            "lm_head", "argmax"};
+                                            "lm_head", "argmax", "paged_plan", "paged_append", "paged_attn",
+                                            "paged_merge"};
 
 // mode 1: one event pair per kernel kind, read after every call (each call waits for its work).
 // mode 2 (deferred): every launch takes the next pair of a per-kind pool and nothing waits, so the
@@ -1607,6 +1610,129 @@ int rbt_hip_matvec(rbt_hip *h, float *out, uint64_t w_offset, const float *x, in
     HIP_OK(h, launch_matvec(lc(h, -1), h->cfg.dtype, h->model + w_offset, x_d, o_d, rows, cols));
     HIP_OK(h, hipMemcpyAsync(out, o_d, (uint64_t)rows * 4, hipMemcpyDeviceToHost, h->stream));
     HIP_OK(h, hipStreamSynchronize(h->stream));
+    return 1;
+}
+
+// ---- the paged key/value cache. The arguments are checked before the handle, so that they can be without a
+// device.
+namespace {
+
+int check_paged_kv(rbt_hip *h, const char *who, const rbt_paged_kv *kv) {
+    if (!kv) return fail(h, "%s: cache descriptor is NULL", who);
+    if (kv->n_blocks < 1 || kv->block_size < 1 || kv->n_kv_heads < 1 || kv->head_dim < 1 || kv->head_dim > kPagedMaxHd ||
+        (int64_t)kv->n_blocks * kv->block_size > INT32_MAX || (int64_t)kv->n_kv_heads * kv->head_dim > (1 << 20))
+        return fail(h, "%s: invalid cache (%d blocks of %d positions, %d heads of %d)", who, kv->n_blocks, kv->block_size,
+                    kv->n_kv_heads, kv->head_dim);
+    if (kv->dtype != RBT_DT_F32 && kv->dtype != RBT_DT_BF16) return fail(h, "%s: invalid dtype %d", who, kv->dtype);
+    if (!kv->k || !kv->v) return fail(h, "%s: cache pointer is NULL", who);
+    const uint64_t block = (uint64_t)kv->n_kv_heads * (uint64_t)kv->block_size * (uint64_t)kv->head_dim;
+    if (kv->block_stride && (kv->block_stride < block || kv->block_stride > UINT64_MAX / 8 / (uint64_t)kv->n_blocks))
+        return fail(h, "%s: block_stride %llu is not between one block (%llu elements) and what can be addressed", who,
+                    (unsigned long long)kv->block_stride, (unsigned long long)block);
+    return 1;
+}
+
+// Heads of a step's rows, and a row stride in floats (0: contiguous).
+int check_paged_heads(rbt_hip *h, const char *who, const rbt_paged_kv *kv, int T, int n_heads) {
+    if (T < 0) return fail(h, "%s: negative token count", who);
+    if (n_heads < 1 || n_heads % kv->n_kv_heads != 0 || (int64_t)n_heads * kv->head_dim > (1 << 20))
+        return fail(h, "%s: %d query heads on %d key/value heads of %d", who, n_heads, kv->n_kv_heads, kv->head_dim);
+    return 1;
+}
+int check_paged_stride(rbt_hip *h, const char *who, const char *name, uint64_t stride, uint64_t row) {
+    if (stride && (stride < row || stride > (1ull << 32)))
+        return fail(h, "%s: %s stride %llu is below the row of %llu floats, or beyond 2^32", who, name,
+                    (unsigned long long)stride, (unsigned long long)row);
+    return 1;
+}
+
+int check_paged_plan(rbt_hip *h, const rbt_paged_plan *p) {
+    if (!p) return fail(h, "paged_plan: plan is NULL");
+    if (p->n_req < 0 || p->n_req > kPagedMaxReq) return fail(h, "paged_plan: n_req %d outside [0, %d]", p->n_req, kPagedMaxReq);
+    if (p->max_blocks < 1 || p->n_blocks < 1 || p->block_size < 1 || p->max_tokens < 0 ||
+        (int64_t)p->max_blocks * p->block_size > INT32_MAX || (int64_t)p->n_blocks * p->block_size > INT32_MAX)
+        return fail(h, "paged_plan: invalid sizes (%d blocks of %d, %d to a request, %d tokens)", p->n_blocks,
+                    p->block_size, p->max_blocks, p->max_tokens);
+    if (!p->n_free || !p->n_free_out || !p->q_start || !p->status || !p->free_list ||
+        (p->n_req > 0 && (!p->len || !p->new_len || !p->tables || !p->kv_len)) ||
+        (p->max_tokens > 0 && (!p->slots || !p->positions)))
+        return fail(h, "paged_plan: NULL array");
+    return 1;
+}
+
+int check_paged_rows(rbt_hip *h, const rbt_paged_kv *kv, const rbt_paged_rows *w) {
+    if (!check_paged_kv(h, "paged_append", kv)) return 0;
+    if (!w) return fail(h, "paged_append: rows descriptor is NULL");
+    if (!check_paged_heads(h, "paged_append", kv, w->n_tokens, w->n_heads)) return 0;
+    const uint64_t qd = (uint64_t)w->n_heads * (uint64_t)kv->head_dim, kvd = (uint64_t)kv->n_kv_heads * (uint64_t)kv->head_dim;
+    if (!check_paged_stride(h, "paged_append", "q", w->q_stride, qd) ||
+        !check_paged_stride(h, "paged_append", "k", w->k_stride, kvd) ||
+        !check_paged_stride(h, "paged_append", "v", w->v_stride, kvd))
+        return 0;
+    if (w->q && w->q_out == w->q && w->q_stride && w->q_stride != qd)
+        return fail(h, "paged_append: q_out is q, whose rows are not contiguous");
+    if (w->rope && (kv->head_dim % 2 != 0 || w->n_rope < 1))
+        return fail(h, "paged_append: rope with head_dim %d, a table of %d positions", kv->head_dim, w->n_rope);
+    if (w->n_tokens > 0 && (!w->k || !w->v || !w->slots || (w->q && !w->q_out) || (w->rope && !w->positions)))
+        return fail(h, "paged_append: NULL array");
+    return 1;
+}
+
+int check_paged_attn(rbt_hip *h, const rbt_paged_kv *kv, const rbt_paged_batch *b, const float *q, uint64_t q_stride, int T,
+                     int n_heads, float scale, int window, const float *out, uint64_t out_stride) {
+    if (!check_paged_kv(h, "paged_attn", kv)) return 0;
+    if (!b) return fail(h, "paged_attn: batch descriptor is NULL");
+    if (b->n_req < 0 || b->n_req > kPagedMaxReq) return fail(h, "paged_attn: n_req %d outside [0, %d]", b->n_req, kPagedMaxReq);
+    if (b->max_blocks < 1 || (int64_t)b->max_blocks * kv->block_size > INT32_MAX)
+        return fail(h, "paged_attn: max_blocks %d (blocks of %d positions)", b->max_blocks, kv->block_size);
+    if (!check_paged_heads(h, "paged_attn", kv, T, n_heads)) return 0;
+    const uint64_t qd = (uint64_t)n_heads * (uint64_t)kv->head_dim;
+    if (!check_paged_stride(h, "paged_attn", "q", q_stride, qd) || !check_paged_stride(h, "paged_attn", "out", out_stride, qd))
+        return 0;
+    if (!isfinite(scale)) return fail(h, "paged_attn: scale is not finite");
+    if (window < 0) return fail(h, "paged_attn: negative window");
+    if (b->n_req > 0 && T > 0 && (!b->tables || !b->kv_len || !b->q_start || !q || !out))
+        return fail(h, "paged_attn: NULL array");
+    return 1;
+}
+
+}  // namespace
+
+int rbt_hip_paged_plan_dev(rbt_hip *h, const rbt_paged_plan *plan) {
+    if (!check_paged_plan(h, plan)) return 0;
+    if (!h) return fail(nullptr, "paged_plan: handle is NULL");
+    if (!set_device(h)) return 0;
+    Launch Lr;  // one event pair per call: the rows' own launch is not timed
+    Lr.s = h->stream;
+    HIP_OK(h, launch_paged_plan(lc(h, kProfPagedPlan), Lr, *plan));
+    return prof_collect(h);
+}
+
+int rbt_hip_paged_append_dev(rbt_hip *h, const rbt_paged_kv *kv, const rbt_paged_rows *rows) {
+    if (!check_paged_rows(h, kv, rows)) return 0;
+    if (!h) return fail(nullptr, "paged_append: handle is NULL");
+    if (rows->n_tokens == 0) return 1;
+    if (!set_device(h)) return 0;
+    HIP_OK(h, launch_paged_append(lc(h, kProfPagedAppend), *kv, *rows));
+    return prof_collect(h);
+}
+
+int rbt_hip_paged_attn_dev(rbt_hip *h, const rbt_paged_kv *kv, const rbt_paged_batch *batch, const float *q,
+                           uint64_t q_stride, int T, int n_heads, float scale, int window, float *out,
+                           uint64_t out_stride) {
+    if (!check_paged_attn(h, kv, batch, q, q_stride, T, n_heads, scale, window, out, out_stride)) return 0;
+    if (!h) return fail(nullptr, "paged_attn: handle is NULL");
+    if (batch->n_req == 0 || T == 0) return 1;
+    if (!set_device(h)) return 0;
+    const uint64_t qd = (uint64_t)n_heads * (uint64_t)kv->head_dim;
+    const float sc = scale == 0.0f ? 1.0f / sqrtf((float)kv->head_dim) : scale;
+    HIP_OK(h, launch_paged_attn(lc(h, kProfPagedAttn), *kv, *batch, q, q_stride ? q_stride : qd, T, n_heads, sc, window, out,
+                                out_stride ? out_stride : qd));
+    return prof_collect(h);
+}
+
+int rbt_hip_paged_reserve(rbt_hip *h) {
+    if (!h) return fail(nullptr, "paged_reserve: handle is NULL");
     return 1;
 }
 

@@ -395,6 +395,15 @@ hipError_t launch_advance(const Launch &L, StepState *st, int B);
 hipError_t launch_record_routing(const Launch &L, const StepState *st, const int32_t *routing, int n_layers, int K,
                                  int B, int ctx, int32_t *hist);
 
+// ---- the paged key/value cache (paged.hip); the arguments are checked (api.hip)
+// Lr: launch context of the rows' own launch, which large steps take.
+hipError_t launch_paged_plan(const Launch &L, const Launch &Lr, const rbt_paged_plan &p);
+hipError_t launch_paged_append(const Launch &L, const rbt_paged_kv &kv, const rbt_paged_rows &w);
+// Strides and scale as given to the kernels (not 0).
+hipError_t launch_paged_attn(const Launch &L, const rbt_paged_kv &kv, const rbt_paged_batch &b, const float *q,
+                             uint64_t q_stride, int T, int n_heads, float scale, int window, float *out,
+                             uint64_t out_stride);
+
 // Dense matvec (one row per wave).
 hipError_t launch_matvec(const Launch &L, int dtype, const void *W, const float *x, float *out, int rows, int cols);
 

@@ -25,7 +25,8 @@ EXPORTS = (
     "rbt_hip_forward_batch", "rbt_hip_generate_batch", "rbt_hip_set_sampling", "rbt_hip_file_info",
     "rbt_hip_generate_stream", "rbt_hip_routing_history", "rbt_hip_expert_cache_replay",
     "rbt_hip_moe_dev_noalloc", "rbt_hip_prefill_layout", "rbt_hip_prefill_layout_drop", "rbt_hip_profiler_attached",
-    "rbt_hip_tile_rows",
+    "rbt_hip_tile_rows", "rbt_hip_paged_plan_dev", "rbt_hip_paged_append_dev", "rbt_hip_paged_attn_dev",
+    "rbt_hip_paged_reserve",
 )
 
 TOKEN_FN = C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_int32)
@@ -42,6 +43,33 @@ class MoeLayer(C.Structure):
     _fields_ = [("dim", C.c_int32), ("n_experts", C.c_int32), ("top_k", C.c_int32), ("expert_hidden", C.c_int32),
                 ("dtype", C.c_int32), ("norm_topk", C.c_int32), ("router", C.c_void_p), ("experts", C.c_void_p),
                 ("expert_stride", C.c_uint64), ("router_bias", C.c_void_p)]
+
+
+class PagedKV(C.Structure):
+    """rbt_paged_kv: one layer's paged key/value cache."""
+    _fields_ = [(n, C.c_int32) for n in ("n_blocks", "block_size", "n_kv_heads", "head_dim", "dtype")] + \
+        [("k", C.c_void_p), ("v", C.c_void_p), ("block_stride", C.c_uint64)]
+
+
+class PagedBatch(C.Structure):
+    """rbt_paged_batch: the requests of a step."""
+    _fields_ = [("n_req", C.c_int32), ("max_blocks", C.c_int32)] + \
+        [(n, C.c_void_p) for n in ("tables", "kv_len", "q_start")]
+
+
+class PagedPlan(C.Structure):
+    """rbt_paged_plan: what a step's plan reads and writes."""
+    _fields_ = [(n, C.c_int32) for n in ("n_req", "max_blocks", "n_blocks", "block_size", "max_tokens")] + \
+        [(n, C.c_void_p) for n in ("len", "new_len", "tables", "free_list", "n_free", "kv_len", "n_free_out", "q_start",
+                                   "slots", "positions", "status")]
+
+
+class PagedRows(C.Structure):
+    """rbt_paged_rows: the rows of a step's new tokens."""
+    _fields_ = [("n_tokens", C.c_int32), ("n_heads", C.c_int32), ("q", C.c_void_p), ("k", C.c_void_p),
+                ("v", C.c_void_p), ("q_stride", C.c_uint64), ("k_stride", C.c_uint64), ("v_stride", C.c_uint64),
+                ("q_out", C.c_void_p), ("q_norm", C.c_void_p), ("k_norm", C.c_void_p), ("eps", C.c_float),
+                ("rope", C.c_void_p), ("n_rope", C.c_int32), ("positions", C.c_void_p), ("slots", C.c_void_p)]
 
 
 class HipError(RuntimeError):
@@ -103,6 +131,11 @@ def lib():
         L.rbt_hip_expert_cache_replay.argtypes = [u64, u64, i32, i32, i32, vp, u64, C.POINTER(C.c_uint64)]
         L.rbt_hip_file_info.argtypes = [C.c_char_p, C.POINTER(Config), C.POINTER(C.c_uint64)]
         L.rbt_hip_profiler_attached.argtypes = []
+        L.rbt_hip_paged_plan_dev.argtypes = [vp, C.POINTER(PagedPlan)]
+        L.rbt_hip_paged_append_dev.argtypes = [vp, C.POINTER(PagedKV), C.POINTER(PagedRows)]
+        L.rbt_hip_paged_attn_dev.argtypes = [vp, C.POINTER(PagedKV), C.POINTER(PagedBatch), vp, u64, i32, i32, f32, i32,
+                                             vp, u64]
+        L.rbt_hip_paged_reserve.argtypes = [vp]
         _lib = L
     return _lib
 
@@ -374,6 +407,22 @@ class Device:
                                               rows, cols))
 
 
+    # ---- the paged key/value cache
+    def paged_plan(self, plan):
+        self._check(self.L.rbt_hip_paged_plan_dev(self.h, C.byref(plan)))
+
+    def paged_append(self, kv, rows):
+        self._check(self.L.rbt_hip_paged_append_dev(self.h, C.byref(kv), C.byref(rows)))
+
+    def paged_attn(self, kv, batch, q, T, n_heads, out, scale=0.0, window=0, q_stride=0, out_stride=0):
+        vp = lambda b: None if b is None else (b if isinstance(b, C.c_void_p) else b.p)
+        self._check(self.L.rbt_hip_paged_attn_dev(self.h, C.byref(kv), C.byref(batch), vp(q), q_stride, T, n_heads, scale,
+                                                  window, vp(out), out_stride))
+
+    def paged_reserve(self):
+        self._check(self.L.rbt_hip_paged_reserve(self.h))
+
+
 def profiler_attached():
     """True while a ROCm profiler tool is attached to this process (rbt_hip_profiler_attached): the
     library then refuses HIP graph replay, and so should a host that captures graphs of its own."""
@@ -393,3 +442,27 @@ def expert_cache_replay(budget_bytes, expert_stride, routing, n_experts):
 def moe_layer_desc(dim, n_experts, top_k, hidden, dtype, norm_topk, router, experts, stride, bias=None):
     ptr = lambda b: None if b is None else (b.value if isinstance(b, C.c_void_p) else b.ptr)
     return MoeLayer(dim, n_experts, top_k, hidden, dtype, norm_topk, ptr(router), ptr(experts), stride, ptr(bias))
+
+
+def _addr(b):
+    return None if b is None else (b.value if isinstance(b, C.c_void_p) else b.ptr)
+
+
+def paged_kv_desc(n_blocks, block_size, n_kv_heads, head_dim, dtype, k, v, block_stride=0):
+    return PagedKV(n_blocks, block_size, n_kv_heads, head_dim, dtype, _addr(k), _addr(v), block_stride)
+
+
+def paged_batch_desc(n_req, max_blocks, tables, kv_len, q_start):
+    return PagedBatch(n_req, max_blocks, _addr(tables), _addr(kv_len), _addr(q_start))
+
+
+def paged_plan_desc(n_req, max_blocks, n_blocks, block_size, max_tokens, len, new_len, tables, free_list, n_free, kv_len,
+                    n_free_out, q_start, slots, positions, status):
+    return PagedPlan(n_req, max_blocks, n_blocks, block_size, max_tokens, *map(_addr, (
+        len, new_len, tables, free_list, n_free, kv_len, n_free_out, q_start, slots, positions, status)))
+
+
+def paged_rows_desc(n_tokens, n_heads, q, k, v, q_out, positions, slots, q_norm=None, k_norm=None, eps=0.0, rope=None,
+                    n_rope=0, q_stride=0, k_stride=0, v_stride=0):
+    return PagedRows(n_tokens, n_heads, _addr(q), _addr(k), _addr(v), q_stride, k_stride, v_stride, _addr(q_out),
+                     _addr(q_norm), _addr(k_norm), eps, _addr(rope), n_rope, _addr(positions), _addr(slots))
