@@ -285,7 +285,8 @@ int rbt_hip_tensor(rbt_hip *h, const char *name, int layer, uint64_t *offset, ui
 
 /* One layer's cache: block b's keys are k + b * block_stride, [n_kv_heads][block_size][head_dim] elements of
  * dtype (RBT_DT_F32 or RBT_DT_BF16), its values v + b * block_stride alike. block_stride 0: blocks follow each
- * other. head_dim 1..256, n_blocks * block_size below 2^31. */
+ * other. head_dim 1..256, n_blocks * block_size below 2^31, max_blocks *
+ * block_size (below) up to 2^31 - 1024. */
 typedef struct {
     int32_t n_blocks, block_size, n_kv_heads, head_dim, dtype;
     void *k, *v;
@@ -363,7 +364,7 @@ int rbt_hip_paged_attn_dev(rbt_hip *h, const rbt_paged_kv *kv, const rbt_paged_b
                            uint64_t q_stride, int T, int n_heads, float scale, int window, float *out,
                            uint64_t out_stride);
 
-/* Allocates the attention's workspace (64 MiB, of one size for every call and held until rbt_hip_free), which the
+/* Allocates the attention's workspace (128 MiB, of one size for every call and held until rbt_hip_free), which the
  * first call does otherwise; needed before capturing one. */
 int rbt_hip_paged_reserve(rbt_hip *h);
 

@@ -165,6 +165,7 @@ struct rbt_hip {
     int tok_host_n = 0;
     // this device's scratch array (rbt_hip_moe_dev_noalloc), from hipGetSymbolAddress at init
     void *scratch = nullptr;
+    void *paged_ws = nullptr;  // the paged attention's workspace (rbt_hip_paged_reserve)
     // tiled copies of layers' experts for the 128-row grouped GEMMs (rbt_hip_prefill_layout), keyed by
     // the layer's expert blobs; built only when the caller asks, used while option "prefill_layout" is on
     std::vector<TiledLayer> tiled;
@@ -487,6 +488,13 @@ Launch lc(rbt_hip *h, int k) {
 }
 
 Launch lc_timed(rbt_hip *h, int k) { return lc(h, k); }
+
+// The handle stream without an event pair: the other launches of a call that is timed by one of them.
+Launch plain(rbt_hip *h) {
+    Launch L;
+    L.s = h->stream;
+    return L;
+}
 
 // Mode 2: waits for the stream and adds the durations of every pair taken since the last read, which
 // frees the pools for reuse.
@@ -1242,6 +1250,7 @@ void rbt_hip_free(rbt_hip *h) {
     (void)hipFree(h->stage);
     if (h->pin) (void)hipHostFree(h->pin);
     (void)hipFree(h->rhist);
+    (void)hipFree(h->paged_ws);
     if (h->tok_host) (void)hipHostFree(h->tok_host);
     tiled_drop(h, nullptr, nullptr);
     (void)hipFree(h->model);
@@ -1634,7 +1643,7 @@ int check_paged_kv(rbt_hip *h, const char *who, const rbt_paged_kv *kv) {
 
 // Heads of a step's rows, and a row stride in floats (0: contiguous).
 int check_paged_heads(rbt_hip *h, const char *who, const rbt_paged_kv *kv, int T, int n_heads) {
-    if (T < 0) return fail(h, "%s: negative token count", who);
+    if (T < 0 || (int64_t)T * n_heads > INT32_MAX) return fail(h, "%s: token count %d (%d heads)", who, T, n_heads);
     if (n_heads < 1 || n_heads % kv->n_kv_heads != 0 || (int64_t)n_heads * kv->head_dim > (1 << 20))
         return fail(h, "%s: %d query heads on %d key/value heads of %d", who, n_heads, kv->n_kv_heads, kv->head_dim);
     return 1;
@@ -1650,7 +1659,7 @@ int check_paged_plan(rbt_hip *h, const rbt_paged_plan *p) {
     if (!p) return fail(h, "paged_plan: plan is NULL");
     if (p->n_req < 0 || p->n_req > kPagedMaxReq) return fail(h, "paged_plan: n_req %d outside [0, %d]", p->n_req, kPagedMaxReq);
     if (p->max_blocks < 1 || p->n_blocks < 1 || p->block_size < 1 || p->max_tokens < 0 ||
-        (int64_t)p->max_blocks * p->block_size > INT32_MAX || (int64_t)p->n_blocks * p->block_size > INT32_MAX)
+        (int64_t)p->max_blocks * p->block_size > kPagedMaxLen || (int64_t)p->n_blocks * p->block_size > INT32_MAX)
         return fail(h, "paged_plan: invalid sizes (%d blocks of %d, %d to a request, %d tokens)", p->n_blocks,
                     p->block_size, p->max_blocks, p->max_tokens);
     if (!p->n_free || !p->n_free_out || !p->q_start || !p->status || !p->free_list ||
@@ -1683,7 +1692,7 @@ int check_paged_attn(rbt_hip *h, const rbt_paged_kv *kv, const rbt_paged_batch *
     if (!check_paged_kv(h, "paged_attn", kv)) return 0;
     if (!b) return fail(h, "paged_attn: batch descriptor is NULL");
     if (b->n_req < 0 || b->n_req > kPagedMaxReq) return fail(h, "paged_attn: n_req %d outside [0, %d]", b->n_req, kPagedMaxReq);
-    if (b->max_blocks < 1 || (int64_t)b->max_blocks * kv->block_size > INT32_MAX)
+    if (b->max_blocks < 1 || (int64_t)b->max_blocks * kv->block_size > kPagedMaxLen)
         return fail(h, "paged_attn: max_blocks %d (blocks of %d positions)", b->max_blocks, kv->block_size);
     if (!check_paged_heads(h, "paged_attn", kv, T, n_heads)) return 0;
     const uint64_t qd = (uint64_t)n_heads * (uint64_t)kv->head_dim;
@@ -1696,15 +1705,24 @@ int check_paged_attn(rbt_hip *h, const rbt_paged_kv *kv, const rbt_paged_batch *
     return 1;
 }
 
+// The attention's workspace: one size for every call, so that it never moves under a captured graph.
+int paged_ws_reserve(rbt_hip *h) {
+    if (h->paged_ws) return 1;
+    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+    HIP_OK(h, hipStreamIsCapturing(h->stream, &cap));
+    if (cap != hipStreamCaptureStatusNone)
+        return fail(h, "paged_attn: the stream is being captured before rbt_hip_paged_reserve");
+    HIP_OK(h, hipMalloc(&h->paged_ws, kPagedWsBytes));
+    return 1;
+}
+
 }  // namespace
 
 int rbt_hip_paged_plan_dev(rbt_hip *h, const rbt_paged_plan *plan) {
     if (!check_paged_plan(h, plan)) return 0;
     if (!h) return fail(nullptr, "paged_plan: handle is NULL");
     if (!set_device(h)) return 0;
-    Launch Lr;  // one event pair per call: the rows' own launch is not timed
-    Lr.s = h->stream;
-    HIP_OK(h, launch_paged_plan(lc(h, kProfPagedPlan), Lr, *plan));
+    HIP_OK(h, launch_paged_plan(lc(h, kProfPagedPlan), plain(h), *plan));
     return prof_collect(h);
 }
 
@@ -1726,14 +1744,15 @@ int rbt_hip_paged_attn_dev(rbt_hip *h, const rbt_paged_kv *kv, const rbt_paged_b
     if (!set_device(h)) return 0;
     const uint64_t qd = (uint64_t)n_heads * (uint64_t)kv->head_dim;
     const float sc = scale == 0.0f ? 1.0f / sqrtf((float)kv->head_dim) : scale;
-    HIP_OK(h, launch_paged_attn(lc(h, kProfPagedAttn), *kv, *batch, q, q_stride ? q_stride : qd, T, n_heads, sc, window, out,
-                                out_stride ? out_stride : qd));
+    if (!paged_ws_reserve(h)) return 0;
+    HIP_OK(h, launch_paged_attn(lc(h, kProfPagedAttn), plain(h), *kv, *batch, q, q_stride ? q_stride : qd, T, n_heads, sc,
+                                window, out, out_stride ? out_stride : qd, h->paged_ws));
     return prof_collect(h);
 }
 
 int rbt_hip_paged_reserve(rbt_hip *h) {
     if (!h) return fail(nullptr, "paged_reserve: handle is NULL");
-    return 1;
+    return set_device(h) && paged_ws_reserve(h);
 }
 
 int rbt_hip_malloc(rbt_hip *h, void **dev, uint64_t bytes) {

@@ -1,6 +1,7 @@
 // Index arithmetic of the paged key/value cache, shared by the kernels (paged.hip) and the host.
 #pragma once
 
+#include <stddef.h>
 #include <stdint.h>
 
 #ifdef __HIPCC__
@@ -14,6 +15,8 @@ namespace rbt {
 
 constexpr int kPagedMaxReq = 4096;   // requests of a step: their prefix sums sit in LDS
 constexpr int kPagedMaxHd = 256;
+constexpr int kPagedMaxLen = 0x7FFFFC00;  // positions of a request's table
+constexpr size_t kPagedWsBytes = 128u << 20;  // the attention's workspace
 
 // n / d for 0 <= n < 2^31 as a product: with s = ceil(log2 d) and m = floor(2^32 (2^s - d) / d) + 1,
 // n / d = (n + high32(n m)) >> s (the sum stays below 2^32, since the product's high half is at most n).

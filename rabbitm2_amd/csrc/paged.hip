@@ -4,6 +4,9 @@
 // row is its own (:472-498).
 #include <math.h>
 
+#include <algorithm>
+#include <atomic>
+
 #include "paged.h"
 #include "rbt2_internal.h"
 
@@ -233,70 +236,840 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
 struct AttnArgs {
     PagedDims d;
     int n_req, max_blocks, T, n_heads, window;
-    float scale;
+    int thin;      // whether requests of up to 16 rows have a launch of their own
+    float scale2;  // scale * log2(e): the softmax runs in powers of two
     const int32_t *tables, *kv_len, *q_start;
     const void *kc, *vc;
     const float *q;
     float *out;
     uint64_t q_stride, out_stride;
+    uint8_t *ws;
 };
 
-// Any head dim and alignment: a block per (row, head), rows and heads in turn; 256 positions at a time, a thread
-// per position for the scores and a thread per dim for the weighted sum, with a running maximum and sum.
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// Softmax state of a set of positions: the reference m (a power of two's exponent; -inf: none seen), the sum l of
+// 2^(s - m) and their weighted values. What a state weighs against the reference M of several:
+__device__ __forceinline__ float state_weight(float m, float M) { return m == -INFINITY ? 0.0f : exp2f(m - M); }
+
+// One (row, head) over positions [j0, j1), by a block of 256 threads and in any head dim: 256 positions at a
+// time, a thread per position for the scores and a thread per dim for the weighted sum. Returns the state, o in
+// thread i < hd. Positions without a place in the cache are not seen, and what they are multiplied with is
+// never read, so no value that is not finite enters from a position that is not seen.
+struct RowShared {
+    uint64_t row[256];
+    float q[kPagedMaxHd], p[256], red[8];
+};
+template <int DT>
+__device__ void row_any(const AttnArgs &a, RowShared &s, int r, int t, int h, int j0, int j1, float *m_out, float *l_out,
+                        float *o_out) {
+    constexpr uint64_t kNone = ~0ull;
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, hd = a.d.hd, kvh = h / (a.n_heads / a.d.n_kv);
+    __syncthreads();  // the shared values of a previous call have been read
+    if (tid < hd) s.q[tid] = a.q[(size_t)t * a.q_stride + (size_t)h * hd + tid];
+    __syncthreads();
+    float m = -INFINITY, l = 0.0f, o = 0.0f;
+    for (; j0 < j1; j0 += 256) {
+        const int j = j0 + tid;
+        float x = -INFINITY;
+        uint64_t row = kNone;
+        if (j < j1) {
+            const int page = (int)page_of((uint32_t)j, a.d.div);
+            const int b = a.tables[(size_t)r * a.max_blocks + page];
+            if (b >= 0 && b < a.d.n_blocks) {
+                row = paged_row(a.d, b, kvh, j - page * a.d.block_size);
+                x = 0.0f;
+                for (int i = 0; i < hd; ++i) x += s.q[i] * load_w<DT>(a.kc, row + i);
+                x *= a.scale2;
+            }
+        }
+        s.row[tid] = row;
+        const float wm = wave_max(x);
+        if (lane == 0) s.red[wv] = wm;
+        __syncthreads();
+        const float mn = fmaxf(fmaxf(m, fmaxf(s.red[0], s.red[1])), fmaxf(s.red[2], s.red[3]));
+        const float ref = mn == -INFINITY ? 0.0f : mn;  // nothing seen yet: all weights 0
+        const float p = row != kNone ? exp2f(x - ref) : 0.0f;
+        s.p[tid] = p;
+        const float ps = wave_sum(p);
+        if (lane == 0) s.red[4 + wv] = ps;
+        __syncthreads();
+        const float alpha = exp2f(m - ref);
+        l = l * alpha + ((s.red[4] + s.red[5]) + (s.red[6] + s.red[7]));
+        o *= alpha;
+        if (tid < hd)
+            for (int jj = 0; jj < min(256, j1 - j0); ++jj)
+                if (s.row[jj] != kNone) o += s.p[jj] * load_w<DT>(a.vc, s.row[jj] + tid);
+        m = mn;
+        __syncthreads();  // red, p and row are rewritten
+    }
+    *m_out = m;
+    *l_out = l;
+    *o_out = o;
+}
+
+// Request r of a step: its new rows m from row t0 on, positions n (p0 before the new ones; negative where the
+// length is below the new rows). Rows outside the step's buffers: the request takes no part (m 0).
+struct Request {
+    int t0, m, n, p0;
+};
+__device__ __forceinline__ Request request(const AttnArgs &a, int r) {
+    Request q;
+    const int t0 = a.q_start[r], t1 = a.q_start[r + 1];
+    q.t0 = t0;
+    q.m = t0 < 0 || t1 > a.T || t1 <= t0 ? 0 : t1 - t0;
+    q.n = min(max(a.kv_len[r], 0), a.max_blocks * a.d.block_size);
+    q.p0 = q.n - q.m;
+    return q;
+}
+
+// Any head dim and alignment: a block per (row, head).
 template <int DT>
 __global__ __launch_bounds__(256) void attn_any_kernel(AttnArgs a) {
-    __shared__ float s_q[kPagedMaxHd], s_p[256], red[8];
-    __shared__ uint64_t s_row[256];
-    constexpr uint64_t kNone = ~0ull;
-    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, hd = a.d.hd;
+    __shared__ RowShared s;
     for (uint64_t id = blockIdx.x; id < (uint64_t)a.T * a.n_heads; id += gridDim.x) {
         const int t = (int)(id / a.n_heads), h = (int)(id % a.n_heads);
         if (t < a.q_start[0]) continue;
-        const int r = request_of(a.q_start, a.n_req, t), t1 = a.q_start[r + 1];
-        if (t >= t1) continue;
-        const int kvh = h / (a.n_heads / a.d.n_kv);
-        const int n = min(max(a.kv_len[r], 0), a.max_blocks * a.d.block_size), pos = n - t1 + t;
-        const int first = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-        __syncthreads();  // the previous row's shared values have been read
-        if (tid < hd) s_q[tid] = a.q[(size_t)t * a.q_stride + (size_t)h * hd + tid];
+        const int r = request_of(a.q_start, a.n_req, t);
+        const Request q = request(a, r);
+        if (t >= q.t0 + q.m) continue;
+        const int pos = q.p0 + t - q.t0, first = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+        float m, l, o;
+        row_any<DT>(a, s, r, t, h, first, pos + 1, &m, &l, &o);
+        if ((int)threadIdx.x < a.d.hd)
+            a.out[(size_t)t * a.out_stride + (size_t)h * a.d.hd + threadIdx.x] = l == 0.0f ? 0.0f : o / l;
+    }
+}
+
+// ---- on the matrix cores (head dims that are multiples of 8, 16-byte aligned rows)
+// Rows: a request's new tokens times the query heads of one key/value head, heads fastest. A tile of rows runs over
+// its positions in tiles, staged in LDS as bf16 parts:
+//   wide   128 rows, 32 to a wave; the block's waves share each tile of keys and values
+//   thin   requests of up to 16 rows (a decoding token) on a bf16 cache: each wave takes tiles of 32 positions
+// in two launches, and long ranges are cut into chunks that different blocks take, joined by a third.
+//
+// Products: v_mfma_f32_16x16x32_bf16, transposed so that nothing moves between lanes: S^T = K Q^T leaves lane
+// (c = l % 16, g = l / 16) the scores of query c with keys 4 g + i of two 16-key groups, which as they stand are
+// the B operand of O^T = V^T P^T whose k-slot (g, 4 t + i) is key 16 t + 4 g + i. V^T comes from the row-major
+// tile by the transposing LDS read (ds_read_b64_tr_b16: lane c of group g gets column c of rows 4 g .. 4 g + 3).
+//
+// Precision: bf16 keys and values enter exactly. f32 operands are cut into three bf16 parts of 8 bits each by
+// truncation (exact for all normal values: 24 bits), and the products of parts down to 2^-24 are taken: three for
+// a bf16 cache, six for an f32 one. Sums, the softmax and its state are f32.
+//
+// Not finite: a position that a row does not see has weight 0, but 0 times an infinity is NaN, so rows whose
+// result is not finite are computed again by row_any, which reads seen positions only. Rows past the positions
+// repeat the last one's, with weight 0.
+constexpr int kWideRows = 128, kThinRows = 16;
+constexpr int kTabPages = 1024;  // block numbers of a chunk held in LDS
+constexpr int kMinChunk = 128, kMaxChunk = kPagedMaxLen;  // positions, multiples of 128
+static_assert(kMaxChunk % 128 == 0, "whole tiles");
+
+// Workspace: for the wide and the thin launch each a header (chunk length, rows to merge) and the prefix sums of the
+// merge rows and of the partial units over the requests, then their partials: units of 16 rows, m [16], l [16],
+// o [16][HDP].
+struct AttnHeader {
+    int32_t chunk, merge_rows, pad[2];
+    int32_t merge[kPagedMaxReq + 4], units[kPagedMaxReq + 4];
+};
+constexpr size_t kWsThin = kPagedWsBytes / 4;  // of it, with its header
+constexpr int unit_floats(int hdp) { return 16 * (hdp + 2); }
+template <bool THIN>
+struct AttnWs {
+    static constexpr size_t kAt = THIN ? 0 : kWsThin, kBytes = THIN ? kWsThin : kPagedWsBytes - kWsThin;
+    __device__ static AttnHeader *header(uint8_t *ws) { return reinterpret_cast<AttnHeader *>(ws + kAt); }
+    __device__ static float *partials(uint8_t *ws) { return reinterpret_cast<float *>(ws + kAt + sizeof(AttnHeader)); }
+    static constexpr int max_units(int hdp) { return (int)((kBytes - sizeof(AttnHeader)) / 4 / unit_floats(hdp)); }
+};
+
+// How a request's rows are cut: tiles of tr rows, each one's positions in nc chunks. rows 0: not this launch's.
+struct Cut {
+    int rows, nt, nc;
+};
+template <bool THIN>
+constexpr int kTileRows = THIN ? kThinRows : kWideRows;
+template <bool THIN>
+__device__ __forceinline__ Cut cut_of(const AttnArgs &a, const Request &q, int chunk) {
+    Cut c;
+    constexpr int tr = kTileRows<THIN>;
+    const int G = a.n_heads / a.d.n_kv;
+    c.rows = q.m * G;
+    if (THIN != (a.thin && c.rows <= kThinRows)) c.rows = 0;
+    c.nt = (c.rows + tr - 1) / tr;
+    // a tile's positions: all up to its last row's, or a window's and what its tokens span
+    const int span = a.window > 0 ? min(q.n, min(a.window, q.n) + (tr - 1) / G + 1) : q.n;
+    c.nc = max(1, (int)(((long long)span + chunk - 1) / chunk));
+    return c;
+}
+
+// Sum over the block's 256 threads and this thread's exclusive prefix.
+__device__ __forceinline__ long long block_scan(long long v, long long *total, long long *s_w) {
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    long long inc = v;
+    for (int off = 1; off < kWave; off <<= 1) {
+        const long long up = __shfl_up(inc, off, kWave);
+        if (lane >= off) inc += up;
+    }
+    __syncthreads();
+    if (lane == kWave - 1) s_w[wv] = inc;
+    __syncthreads();
+    long long before = 0;
+    for (int w = 0; w < wv; ++w) before += s_w[w];
+    *total = (s_w[0] + s_w[1]) + (s_w[2] + s_w[3]);
+    return before + inc - v;
+}
+
+// A launch's items (request, head, row tile, chunk), by every block for itself: prefix sums over the requests into
+// s_items [n_req + 1] and s_units. The chunk length spreads the work over about two rounds of blocks; it doubles
+// until the partials fit, which ends at the latest at kMaxChunk, where no tile is cut.
+template <bool THIN>
+__device__ int schedule(const AttnArgs &a, int units_max, int32_t *s_items, int32_t *s_units,
+                        long long *s_w) {
+    const int per = (a.n_req + 255) / 256, r0 = min(a.n_req, (int)threadIdx.x * per), r1 = min(a.n_req, r0 + per);
+    long long work = 0, total;
+    for (int r = r0; r < r1; ++r) {
+        const Request q = request(a, r);
+        if (!q.m) continue;
+        const Cut c = cut_of<THIN>(a, q, kMaxChunk);
+        work += (long long)c.nt * (a.window > 0 ? min(q.n, min(a.window, q.n) + kTileRows<THIN>) : q.n - q.m / 2);
+    }
+    block_scan(work, &total, s_w);
+    long long chunk = (total * a.d.n_kv / (2 * gridDim.x) + 127) / 128 * 128;
+    chunk = min(max(chunk, (long long)kMinChunk), (long long)kMaxChunk);
+    for (;;) {
+        long long items = 0, units = 0, merge = 0;
+        for (int r = r0; r < r1; ++r) {
+            const Request q = request(a, r);
+            if (!q.m) continue;
+            const Cut c = cut_of<THIN>(a, q, (int)chunk);
+            const long long n = (long long)c.nt * a.d.n_kv * c.nc;
+            items += n;
+            if (c.nc > 1) {
+                units += n * (kTileRows<THIN> / 16);
+                merge += (long long)c.rows * a.d.n_kv;
+            }
+        }
+        long long n_items, n_units, n_merge;
+        long long i0 = block_scan(items, &n_items, s_w), u0 = block_scan(units, &n_units, s_w);
+        if (n_units > units_max && chunk < kMaxChunk) {
+            chunk = min(2 * chunk, (long long)kMaxChunk);
+            continue;
+        }
+        long long m0 = 0;
+        AttnHeader *hdr = blockIdx.x == 0 ? AttnWs<THIN>::header(a.ws) : nullptr;  // one block tells the merge launch
+        if (hdr) m0 = block_scan(merge, &n_merge, s_w);
+        for (int r = r0; r < r1; ++r) {
+            s_items[r] = (int)i0;
+            s_units[r] = (int)u0;
+            if (hdr) {
+                hdr->merge[r] = (int)m0;
+                hdr->units[r] = (int)u0;
+            }
+            const Request q = request(a, r);
+            if (!q.m) continue;
+            const Cut c = cut_of<THIN>(a, q, (int)chunk);
+            const long long n = (long long)c.nt * a.d.n_kv * c.nc;
+            i0 += n;
+            if (c.nc > 1) {
+                u0 += n * (kTileRows<THIN> / 16);
+                m0 += (long long)c.rows * a.d.n_kv;
+            }
+        }
+        if (threadIdx.x == 0) {
+            s_items[a.n_req] = (int)n_items;
+            if (hdr) {
+                hdr->chunk = (int)chunk;
+                hdr->merge_rows = (int)n_merge;
+            }
+        }
         __syncthreads();
-        float m = -INFINITY, l = 0.0f, o = 0.0f;
-        for (int j0 = first; j0 <= pos; j0 += 256) {
-            const int j = j0 + tid;
-            float s = -INFINITY;
-            uint64_t row = kNone;
-            if (j <= pos) {
-                const int page = (int)page_of((uint32_t)j, a.d.div);
-                const int b = a.tables[(size_t)r * a.max_blocks + page];
-                if (b >= 0 && b < a.d.n_blocks) {
-                    row = paged_row(a.d, b, kvh, j - page * a.d.block_size);
-                    s = 0.0f;
-                    for (int i = 0; i < hd; ++i) s += s_q[i] * load_w<DT>(a.kc, row + i);
-                    s *= a.scale;
+        return (int)chunk;
+    }
+}
+
+// Two f32 as packed bf16 by truncation, and what that leaves of them.
+__device__ __forceinline__ uint32_t take_part(float &x, float &y) {
+    const uint32_t ux = __float_as_uint(x), uy = __float_as_uint(y);
+    x -= __uint_as_float(ux & 0xFFFF0000u);
+    y -= __uint_as_float(uy & 0xFFFF0000u);
+    return __builtin_amdgcn_perm(uy, ux, 0x07060302u);
+}
+// Eight f32 in three parts.
+__device__ __forceinline__ void split3(float (&x)[8], u32x4 (&part)[3]) {
+#pragma unroll
+    for (int p = 0; p < 3; ++p)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) part[p][i] = take_part(x[2 * i], x[2 * i + 1]);
+}
+
+// max and sum over the four lanes of a query
+__device__ __forceinline__ float group_max(float v) {
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float group_sum(float v) {
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// LDS layout of a tile part: rows of HDP bf16 and 16 bytes more, so that the same chunk of 16 rows (a K operand) and
+// the same 32 bytes of 16 rows (V^T) lie in all banks evenly, at fixed distances from a lane's first.
+template <int HDP>
+constexpr int kTileRow = HDP * 2 + 16;
+
+extern __shared__ __align__(16) uint8_t smem[];
+
+// What a wave keeps of its NQ * 16 rows.
+template <int HDP, int NQ>
+struct WaveState {
+    u32x4 q[NQ][HDP / 32][3];
+    f32x4 o[NQ][HDP / 16];
+    float m[NQ], l[NQ];
+    int pos[NQ];  // this lane's query's position
+};
+
+// 32 positions, rows row0 .. row0 + 31 of the staged tile (keys at byte k_off of LDS, values at v_off, parts
+// `part` bytes apart); seen(n): bit 4 t + i, whether query n of this lane sees key 16 t + 4 g + i of them
+// (asked where !full).
+template <int HDP, int NQ, int NP, int part, typename Seen>
+__device__ __forceinline__ void attn_step(WaveState<HDP, NQ> &w, int k_off, int v_off, int row0, float scale2,
+                                          bool full, Seen seen) {
+    constexpr int RS = kTileRow<HDP>;
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    const int k_at = k_off + (row0 + c) * RS + 16 * g, v_at = v_off + (row0 + 4 * g + (c >> 2)) * RS + 8 * (c & 3);
+    f32x4 s[NQ][2];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) s[n][0] = s[n][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int st = 0; st < HDP / 32; ++st) {
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int kp = 0; kp < NP; ++kp) {
+                const u32x4 k = *reinterpret_cast<const u32x4 *>(smem + k_at + kp * part + t * 16 * RS + st * 64);
+#pragma unroll
+                for (int qp = 0; qp + kp < 3; ++qp)
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n) s[n][t] = mfma(k, w.q[n][st][qp], s[n][t]);
+            }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (!full) {
+        const float none = scale2 < 0.0f ? INFINITY : -INFINITY;  // weight 0
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            const uint32_t bits = seen(n);
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[n][t][i] = bits >> (4 * t + i) & 1 ? s[n][t][i] : none;
+        }
+    }
+    // The reference moves only when a score is 2^8 above it (weights stay below 2^8 then): most steps neither
+    // reduce over the lanes nor rescale.
+    float top[NQ];
+    bool move = false;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        top[n] = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top[n] = fmaxf(top[n], s[n][t][i] * scale2);
+        move |= top[n] > w.m[n] + 8.0f;
+    }
+    if (__any(move)) {
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            const float m = fmaxf(w.m[n], group_max(top[n]));
+            const float a = w.m[n] == -INFINITY ? 0.0f : exp2f(w.m[n] - m);
+            w.m[n] = m;
+            w.l[n] *= a;
+#pragma unroll
+            for (int d = 0; d < HDP / 16; ++d) w.o[n][d] *= a;
+        }
+    }
+    u32x4 p[NQ][3];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        const float ref = w.m[n] == -INFINITY ? 0.0f : w.m[n];
+        float e[8];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                e[4 * t + i] = __builtin_amdgcn_exp2f(fmaf(s[n][t][i], scale2, -ref));
+                w.l[n] += e[4 * t + i];
+            }
+        split3(e, p[n]);
+    }
+#pragma unroll
+    for (int d = 0; d < HDP / 16; ++d) {
+        if (d % 2 == 0) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int vp = 0; vp < NP; ++vp) {
+            u32x4 v;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const u32x2 h = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (__attribute__((address_space(3))) s16x4 *)(smem + v_at + vp * part + t * 16 * RS + d * 32)));
+                v[2 * t] = h[0];
+                v[2 * t + 1] = h[1];
+            }
+#pragma unroll
+            for (int pp = 0; pp + vp < 3; ++pp)
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) w.o[n][d] = mfma(v, p[n][pp], w.o[n][d]);
+        }
+    }
+}
+
+// The rows of a wave: rows row0 .. row0 + 16 NQ - 1 of the request (clamped to its last), q in three parts.
+template <int HDP, int NQ>
+__device__ __forceinline__ void wave_init(WaveState<HDP, NQ> &w, const AttnArgs &a, const Request &q, int rows, int kvh,
+                                          int row0) {
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, G = a.n_heads / a.d.n_kv;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        const int row = min(row0 + 16 * n + c, rows - 1), tok = row / G, h = kvh * G + row - tok * G;
+        const float *src = a.q + (size_t)(q.t0 + tok) * a.q_stride + (size_t)h * a.d.hd + 8 * g;
+        w.pos[n] = q.p0 + tok;
+        w.m[n] = -INFINITY;
+        w.l[n] = 0.0f;
+#pragma unroll
+        for (int st = 0; st < HDP / 32; ++st) {
+            float x[8];
+            const bool in = 32 * st + 8 * g < a.d.hd;
+            const f32x4 x0 = in ? ld_f4(src + 32 * st) : f32x4{0.0f, 0.0f, 0.0f, 0.0f},
+                        x1 = in ? ld_f4(src + 32 * st + 4) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[i] = x0[i];
+                x[4 + i] = x1[i];
+            }
+            split3(x, w.q[n][st]);
+        }
+#pragma unroll
+        for (int d = 0; d < HDP / 16; ++d) w.o[n][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+}
+
+// Staging of KEYS positions from j on (those past last repeat it) by THREADS threads: 16-byte chunks of 8 elements
+// through registers, so that a tile's loads run during the arithmetic of the one before.
+template <int DT, int HDP, int KEYS, int THREADS>
+struct Stage {
+    static constexpr int CH = HDP / 8, ROWS = THREADS / CH, N = KEYS / ROWS;
+    static constexpr int LD = DT == RBT_DT_BF16 ? 1 : 2;
+    static_assert(N * ROWS == KEYS, "whole passes");
+    u32x4 k[N][LD], v[N][LD];
+
+    __device__ __forceinline__ void load(const AttnArgs &a, const int32_t *s_tab, int page0, int kvh, int j, int last,
+                                         int tid) {
+        const int row = tid / CH, chunk = tid % CH;
+        const bool in = 8 * chunk < a.d.hd;
+        constexpr size_t esz = DT == RBT_DT_BF16 ? 2 : 4;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int key = min(j + row + i * ROWS, last), page = (int)page_of((uint32_t)key, a.d.div);
+            const int b = max(s_tab[page - page0], 0);
+            const uint64_t at = (paged_row(a.d, b, kvh, key - page * a.d.block_size) + 8 * chunk) * esz;
+#pragma unroll
+            for (int x = 0; x < LD; ++x) {
+                k[i][x] = v[i][x] = u32x4{0, 0, 0, 0};
+                if (in) {
+                    k[i][x] = *reinterpret_cast<const u32x4 *>(static_cast<const uint8_t *>(a.kc) + at + 16 * x);
+                    v[i][x] = *reinterpret_cast<const u32x4 *>(static_cast<const uint8_t *>(a.vc) + at + 16 * x);
                 }
             }
-            s_row[tid] = row;
-            const float wm = wave_max(s);
-            if (lane == 0) red[wv] = wm;
-            __syncthreads();
-            const float mn = fmaxf(fmaxf(m, fmaxf(red[0], red[1])), fmaxf(red[2], red[3]));
-            const float ref = mn == -INFINITY ? 0.0f : mn;  // nothing seen yet: all weights 0
-            const float p = row != kNone ? expf(s - ref) : 0.0f;
-            s_p[tid] = p;
-            const float ps = wave_sum(p);
-            if (lane == 0) red[4 + wv] = ps;
-            __syncthreads();
-            const float alpha = expf(m - ref);
-            l = l * alpha + ((red[4] + red[5]) + (red[6] + red[7]));
-            o *= alpha;
-            if (tid < hd)
-                for (int jj = 0; jj < min(256, pos + 1 - j0); ++jj)
-                    if (s_row[jj] != kNone) o += s_p[jj] * load_w<DT>(a.vc, s_row[jj] + tid);
-            m = mn;
-            __syncthreads();  // red, s_p and s_row are rewritten
         }
-        if (tid < hd) a.out[(size_t)t * a.out_stride + (size_t)h * hd + tid] = l == 0.0f ? 0.0f : o / l;
     }
+    __device__ __forceinline__ void put(const u32x4 (&r)[LD], int off, int part) {
+        if constexpr (DT == RBT_DT_BF16) {
+            *reinterpret_cast<u32x4 *>(smem + off) = r[0];
+        } else {
+            float x[8];
+            u32x4 p[3];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(r[i / 4][i % 4]);
+            split3(x, p);
+#pragma unroll
+            for (int y = 0; y < 3; ++y) *reinterpret_cast<u32x4 *>(smem + off + y * part) = p[y];
+        }
+    }
+    __device__ __forceinline__ void store(int k_off, int v_off, int part, int tid) {
+        const int at = tid / CH * kTileRow<HDP> + 16 * (tid % CH);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int off = at + i * ROWS * kTileRow<HDP>;
+            put(k[i], k_off + off, part);
+            put(v[i], v_off + off, part);
+        }
+    }
+};
+
+// A row's place: its token and head.
+struct Place {
+    int t, h, pos;
+};
+__device__ __forceinline__ Place place(const AttnArgs &a, const Request &q, int kvh, int row) {
+    const int G = a.n_heads / a.d.n_kv, tok = row / G;
+    return {q.t0 + tok, kvh * G + row - tok * G, q.p0 + tok};
+}
+
+// A launch's item.
+struct Item {
+    Request q;
+    Cut cut;
+    int r, kvh, row0, n_rows, pa, pb, k0, k1;  // rows row0 .. row0 + n_rows - 1 at positions pa .. pb; chunk [k0, k1)
+    float *unit;                               // its partials
+};
+template <bool THIN, int HDP>
+__device__ __forceinline__ Item item_of(const AttnArgs &a, int it, int chunk, const int32_t *s_items,
+                                        const int32_t *s_units) {
+    constexpr int tr = kTileRows<THIN>;
+    Item x;
+    // the same for all threads, told to the compiler
+    x.r = __builtin_amdgcn_readfirstlane(request_of(s_items, a.n_req, it));
+    x.q = request(a, x.r);
+    x.cut = cut_of<THIN>(a, x.q, chunk);
+    int local = it - __builtin_amdgcn_readfirstlane(s_items[x.r]);
+    const int c = local % x.cut.nc;
+    local /= x.cut.nc;
+    x.kvh = local / x.cut.nt;
+    const int tile = x.cut.nt - 1 - local % x.cut.nt;  // the longest tiles first
+    x.row0 = tile * tr;
+    x.n_rows = min(tr, x.cut.rows - x.row0);
+    x.pa = place(a, x.q, x.kvh, x.row0).pos;
+    x.pb = place(a, x.q, x.kvh, x.row0 + x.n_rows - 1).pos;
+    const int lo = a.window > 0 ? max(0, x.pa - a.window + 1) : 0;
+    x.k0 = (int)min((long long)lo + (long long)c * chunk, (long long)kPagedMaxLen);
+    x.k1 = min(x.pb + 1, (int)min((long long)x.k0 + chunk, (long long)kPagedMaxLen));
+    x.unit = AttnWs<THIN>::partials(a.ws) +
+             ((size_t)__builtin_amdgcn_readfirstlane(s_units[x.r]) +
+              ((size_t)(x.kvh * x.cut.nt + tile) * x.cut.nc + c) * (tr / 16)) * unit_floats(HDP);
+    return x;
+}
+// Items in order of (request, head, tile, chunk); an eighth of them to each XCD (blocks b % 8), so that a head's row
+// tiles read its keys and values through one L2.
+struct ItemRange {
+    int first, end, step;
+};
+__device__ __forceinline__ ItemRange item_range(int n_items) {
+    const int xcd = blockIdx.x & 7;
+    const int i0 = (int)((long long)n_items * xcd / 8), i1 = (int)((long long)n_items * (xcd + 1) / 8);
+    return {i0 + (int)(blockIdx.x >> 3), i1, (int)(gridDim.x >> 3)};
+}
+
+// Block numbers of the pages that positions j0 .. j1 - 1 (at most tab_span of them) lie on, into s_tab; -1 for one
+// outside the cache: whether there is any. For all threads of the block.
+constexpr int kTabBytes = 4 * kTabPages;
+__device__ __forceinline__ int tab_span(const AttnArgs &a) {
+    return (int)(min((kTabPages - 1) * (long long)a.d.block_size, (long long)kMaxChunk) / 128 * 128);
+}
+__device__ __forceinline__ bool fill_tab(const AttnArgs &a, int r, int j0, int j1, int32_t *s_tab) {
+    const int page0 = (int)page_of((uint32_t)j0, a.d.div), n = (int)page_of((uint32_t)(j1 - 1), a.d.div) - page0 + 1;
+    bool bad = false;
+    __syncthreads();  // the last table has been read
+    for (int i = threadIdx.x; i < n; i += 256) {
+        const int b = a.tables[(size_t)r * a.max_blocks + page0 + i];
+        const bool ok = b >= 0 && b < a.d.n_blocks;
+        bad |= !ok;
+        s_tab[i] = ok ? b : -1;
+    }
+    return __builtin_amdgcn_readfirstlane(__syncthreads_or(bad)) != 0;
+}
+
+// Which of a lane's 16 t + 4 g + i (bit 4 t + i) of 32 positions from j on the query at pos sees.
+__device__ __forceinline__ uint32_t seen_bits(const AttnArgs &a, int j, int k1, int pos, const int32_t *s_tab, int page0,
+                                              bool bad) {
+    const int g = (threadIdx.x & 63) >> 4;
+    const int first = a.window > 0 ? pos - a.window : -1, last = min(k1 - 1, pos);
+    uint32_t bits = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int key = j + 16 * (e >> 2) + 4 * g + (e & 3);
+        bits |= (uint32_t)((key <= last) & (key > first)) << e;
+    }
+    if (bad)
+        for (int e = 0; e < 8; ++e) {
+            const int key = min(j + 16 * (e >> 2) + 4 * g + (e & 3), k1 - 1);
+            if (s_tab[(int)page_of((uint32_t)key, a.d.div) - page0] < 0) bits &= ~(1u << e);
+        }
+    return bits;
+}
+
+// The flagged rows of an item again, one by one.
+template <int DT, int HDP>
+__device__ __forceinline__ void again_rows(const AttnArgs &a, const Item &x, const int *s_flag) {
+    for (int row = 0; row < x.n_rows; ++row) {
+        if (!s_flag[row]) continue;  // the same for all threads
+        const Place pl = place(a, x.q, x.kvh, x.row0 + row);
+        const int j0 = a.window > 0 ? max(x.k0, pl.pos - a.window + 1) : x.k0;
+        float m, l, o;
+        row_any<DT>(a, *reinterpret_cast<RowShared *>(smem), x.r, pl.t, pl.h, j0, min(x.k1, pl.pos + 1), &m, &l, &o);
+        if (x.cut.nc > 1) {
+            float *un = x.unit + (size_t)(row >> 4) * unit_floats(HDP);
+            if (threadIdx.x == 0) {
+                un[row & 15] = m;
+                un[16 + (row & 15)] = l;
+            }
+            if (threadIdx.x < HDP) un[32 + (row & 15) * HDP + threadIdx.x] = (int)threadIdx.x < a.d.hd ? o : 0.0f;
+        } else if ((int)threadIdx.x < a.d.hd) {
+            a.out[(size_t)pl.t * a.out_stride + (size_t)pl.h * a.d.hd + threadIdx.x] = l == 0.0f ? 0.0f : o / l;
+        }
+    }
+}
+
+// LDS: [tile | row_any's][block numbers][item and unit prefix sums]
+constexpr int kLdsBytes = 159 << 10;  // of 160 KiB: the kernels' fixed shared variables take less than the last
+constexpr int attn_lds(int tile, int n_req) { return tile + kTabBytes + 8 * (n_req + 1); }
+
+// Requests of up to 16 rows.
+template <int HDP>
+struct ThinShape {
+    static constexpr int WAVE = 2 * 32 * kTileRow<HDP>;  // a wave's own keys and values, and later its rows
+    static constexpr int TILE = 4 * WAVE;
+    static constexpr int PER_CU = HDP <= 128 ? 2 : 1;  // blocks that share a CU
+    static_assert(kThinRows * (HDP + 4) * 4 <= WAVE, "a wave's rows fit its tile");
+    static_assert(sizeof(RowShared) <= (size_t)TILE, "row_any's LDS");
+};
+template <int HDP>
+__global__ __launch_bounds__(256, (ThinShape<HDP>::PER_CU)) void attn_thin_kernel(AttnArgs a) {
+    constexpr int DT = RBT_DT_BF16, WAVE = ThinShape<HDP>::WAVE;
+    __shared__ long long s_w[4];
+    __shared__ float s_m[4][kThinRows], s_l[4][kThinRows];
+    __shared__ int s_flag[kThinRows];
+    int32_t *s_tab = reinterpret_cast<int32_t *>(smem + ThinShape<HDP>::TILE), *s_items = s_tab + kTabPages,
+            *s_units = s_items + a.n_req + 1;
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
+    const int chunk = __builtin_amdgcn_readfirstlane(
+        schedule<true>(a, AttnWs<true>::max_units(HDP), s_items, s_units, s_w));
+    const ItemRange items = item_range(__builtin_amdgcn_readfirstlane(s_items[a.n_req]));
+    const int span = tab_span(a);
+    for (int it = items.first; it < items.end; it += items.step) {
+        const Item x = item_of<true, HDP>(a, it, chunk, s_items, s_units);
+        WaveState<HDP, 1> w;
+        wave_init<HDP, 1>(w, a, x.q, x.cut.rows, x.kvh, x.row0);
+        const int k_off = wv * WAVE, v_off = k_off + 32 * kTileRow<HDP>;
+        for (int w0 = x.k0; w0 < x.k1; w0 += span) {
+            const int w1 = min(x.k1, w0 + min(span, x.k1 - w0)), page0 = (int)page_of((uint32_t)w0, a.d.div);
+            const bool bad = fill_tab(a, x.r, w0, w1, s_tab);
+            Stage<DT, HDP, 32, 64> st;
+            int j = w0 + 32 * wv;
+            if (j < w1) st.load(a, s_tab, page0, x.kvh, j, w1 - 1, lane);
+            for (; j < w1; j += 128) {
+                __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+                st.store(k_off, v_off, 0, lane);
+                __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+                if (j + 128 < w1) st.load(a, s_tab, page0, x.kvh, j + 128, w1 - 1, lane);
+                const bool full = !bad && j + 32 <= min(w1, x.pa + 1) && (a.window <= 0 || j > x.pb - a.window);
+                attn_step<HDP, 1, 1, 0>(w, k_off, v_off, 0, a.scale2, full,
+                                        [&](int n) { return seen_bits(a, j, w1, w.pos[n], s_tab, page0, bad); });
+            }
+        }
+        // the four waves' states, joined; each wave's rows lie where its tile was
+        const bool split = x.cut.nc > 1;
+        w.l[0] = group_sum(w.l[0]);
+        if (g == 0) {
+            s_m[wv][c] = w.m[0];
+            s_l[wv][c] = w.l[0];
+        }
+        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+#pragma unroll
+        for (int d = 0; d < HDP / 16; ++d)
+            *reinterpret_cast<f32x4 *>(smem + k_off + (c * (HDP + 4) + 16 * d + 4 * g) * 4) = w.o[0][d];
+        if (tid < kThinRows) s_flag[tid] = 0;
+        __syncthreads();
+        const int row = tid >> 4, y = tid & 15;
+        float M = -INFINITY, L = 0.0f, wt[4];
+#pragma unroll
+        for (int z = 0; z < 4; ++z) M = fmaxf(M, s_m[z][row]);
+#pragma unroll
+        for (int z = 0; z < 4; ++z) {
+            wt[z] = state_weight(s_m[z][row], M);
+            L += wt[z] * s_l[z][row];
+        }
+        f32x4 o[HDP / 64];
+        float nan = 0.0f * L;
+#pragma unroll
+        for (int u = 0; u < HDP / 64; ++u) {
+            o[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int z = 0; z < 4; ++z)
+                o[u] += wt[z] * *reinterpret_cast<const f32x4 *>(smem + z * WAVE + (row * (HDP + 4) + 64 * u + 4 * y) * 4);
+            nan += 0.0f * ((o[u].x + o[u].y) + (o[u].z + o[u].w));
+        }
+        const bool again = ((__ballot(nan != 0.0f) >> (lane & 48)) & 0xFFFFu) != 0;
+        if (row < x.n_rows) {
+            if (again) {
+                if (y == 0) s_flag[row] = 1;
+            } else if (split) {
+                if (y == 0) {
+                    x.unit[row] = M;
+                    x.unit[16 + row] = L;
+                }
+#pragma unroll
+                for (int u = 0; u < HDP / 64; ++u)
+                    *reinterpret_cast<f32x4 *>(x.unit + 32 + row * HDP + 64 * u + 4 * y) = o[u];
+            } else {
+                const Place pl = place(a, x.q, x.kvh, x.row0 + row);
+                float *dst = a.out + (size_t)pl.t * a.out_stride + (size_t)pl.h * a.d.hd;
+                const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+#pragma unroll
+                for (int u = 0; u < HDP / 64; ++u)
+                    if (64 * u + 4 * y < a.d.hd) *reinterpret_cast<f32x4 *>(dst + 64 * u + 4 * y) = o[u] * inv;
+            }
+        }
+        if (__syncthreads_or(again && row < x.n_rows)) again_rows<DT, HDP>(a, x, s_flag);
+        __syncthreads();
+    }
+}
+
+// The other requests.
+template <int DT, int HDP>
+struct WideShape {
+    static constexpr int NP = DT == RBT_DT_BF16 ? 1 : 3;
+    static constexpr int KEYS = DT == RBT_DT_BF16 && HDP <= 128 ? 64 : 32;
+    static constexpr int PART = KEYS * kTileRow<HDP>;
+    static constexpr int TILE = 2 * NP * PART;
+    static constexpr int PER_CU = HDP <= 128 ? 2 : 1;
+    static_assert(sizeof(RowShared) <= (size_t)TILE, "row_any's LDS");
+};
+template <int DT, int HDP>
+__global__ __launch_bounds__(256, (WideShape<DT, HDP>::PER_CU)) void attn_wide_kernel(AttnArgs a) {
+    using Sh = WideShape<DT, HDP>;
+    __shared__ long long s_w[4];
+    __shared__ int s_flag[kWideRows];
+    int32_t *s_tab = reinterpret_cast<int32_t *>(smem + Sh::TILE), *s_items = s_tab + kTabPages,
+            *s_units = s_items + a.n_req + 1;
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
+    const int chunk = __builtin_amdgcn_readfirstlane(
+        schedule<false>(a, AttnWs<false>::max_units(HDP), s_items, s_units, s_w));
+    const ItemRange items = item_range(__builtin_amdgcn_readfirstlane(s_items[a.n_req]));
+    const int span = tab_span(a);
+    for (int it = items.first; it < items.end; it += items.step) {
+        const Item x = item_of<false, HDP>(a, it, chunk, s_items, s_units);
+        if (x.k0 >= x.k1 && x.k0 > 0) continue;  // a chunk behind the tile's positions: the merge knows
+        const int wr0 = x.row0 + 32 * wv;
+        const bool active = 32 * wv < x.n_rows;
+        const int wa = place(a, x.q, x.kvh, min(wr0, x.cut.rows - 1)).pos,
+                  wb = place(a, x.q, x.kvh, min(wr0 + 31, x.cut.rows - 1)).pos;
+        WaveState<HDP, 2> w;
+        wave_init<HDP, 2>(w, a, x.q, x.cut.rows, x.kvh, wr0);
+        constexpr int k_off = 0, v_off = Sh::NP * Sh::PART;
+        for (int w0 = x.k0; w0 < x.k1; w0 += span) {
+            const int w1 = min(x.k1, w0 + min(span, x.k1 - w0)), page0 = (int)page_of((uint32_t)w0, a.d.div);
+            const bool bad = fill_tab(a, x.r, w0, w1, s_tab);
+            Stage<DT, HDP, Sh::KEYS, 256> st;
+            st.load(a, s_tab, page0, x.kvh, w0, w1 - 1, tid);
+            for (int jt = w0; jt < w1; jt += Sh::KEYS) {
+                __syncthreads();
+                st.store(k_off, v_off, Sh::PART, tid);
+                __syncthreads();
+                if (jt + Sh::KEYS < w1) st.load(a, s_tab, page0, x.kvh, jt + Sh::KEYS, w1 - 1, tid);
+                for (int u = 0; u < Sh::KEYS; u += 32) {
+                    const int j = jt + u;
+                    if (!active || j >= w1 || j > wb || (a.window > 0 && j + 31 <= wa - a.window)) continue;
+                    const bool full = !bad && j + 32 <= min(w1, wa + 1) && (a.window <= 0 || j > wb - a.window);
+                    attn_step<HDP, 2, Sh::NP, Sh::PART>(
+                        w, k_off, v_off, u, a.scale2, full,
+                        [&](int n) { return seen_bits(a, j, w1, w.pos[n], s_tab, page0, bad); });
+                }
+            }
+        }
+        const bool split = x.cut.nc > 1;
+        if (tid < kWideRows) s_flag[tid] = 0;
+        __syncthreads();
+        bool any = false;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const int row = 32 * wv + 16 * n + c;
+            const float L = group_sum(w.l[n]);
+            float nan = 0.0f * L;
+#pragma unroll
+            for (int d = 0; d < HDP / 16; ++d)
+                nan += 0.0f * ((w.o[n][d].x + w.o[n][d].y) + (w.o[n][d].z + w.o[n][d].w));
+            const bool again = ((__ballot(nan != 0.0f) >> c) & 0x0001000100010001ull) != 0;
+            if (row >= x.n_rows) continue;
+            if (again) {
+                s_flag[row] = 1;
+                any = true;
+            } else if (split) {
+                float *un = x.unit + (size_t)(row >> 4) * unit_floats(HDP);
+                if (g == 0) {
+                    un[c] = w.m[n];
+                    un[16 + c] = L;
+                }
+#pragma unroll
+                for (int d = 0; d < HDP / 16; ++d)
+                    *reinterpret_cast<f32x4 *>(un + 32 + c * HDP + 16 * d + 4 * g) = w.o[n][d];
+            } else {
+                const Place pl = place(a, x.q, x.kvh, x.row0 + row);
+                float *dst = a.out + (size_t)pl.t * a.out_stride + (size_t)pl.h * a.d.hd + 4 * g;
+                const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+#pragma unroll
+                for (int d = 0; d < HDP / 16; ++d)
+                    if (16 * d + 4 * g < a.d.hd) *reinterpret_cast<f32x4 *>(dst + 16 * d) = w.o[n][d] * inv;
+            }
+        }
+        if (__syncthreads_or(any)) again_rows<DT, HDP>(a, x, s_flag);
+        __syncthreads();
+    }
+}
+
+// The chunks of cut tiles joined, a wave per row: out = sum_i w_i o_i / sum_i w_i l_i with w_i = 2^(m_i - max m).
+template <int HDP, bool THIN>
+__device__ __forceinline__ void merge_row(const AttnArgs &a, const AttnHeader *hdr, int id) {
+    constexpr int tr = kTileRows<THIN>, tru = tr / 16, VL = HDP / 64;  // VL: floats per lane
+    const int lane = threadIdx.x & 63, r = request_of(hdr->merge, a.n_req, id), chunk = hdr->chunk;
+    const Request q = request(a, r);
+    const Cut cut = cut_of<THIN>(a, q, chunk);
+    const int local = id - hdr->merge[r], kvh = local / cut.rows, row = local - kvh * cut.rows, tile = row / tr;
+    const int row0 = tile * tr, n_rows = min(tr, cut.rows - row0), in = row - row0;
+    const int pa = place(a, q, kvh, row0).pos, pb = place(a, q, kvh, row0 + n_rows - 1).pos;
+    const int lo = a.window > 0 ? max(0, pa - a.window + 1) : 0;
+    const int nc = max(1, min(cut.nc, (int)(((long long)pb + 1 - lo + chunk - 1) / chunk)));  // those that hold positions
+    const float *u = AttnWs<THIN>::partials(a.ws) +
+                     ((size_t)hdr->units[r] + (size_t)(kvh * cut.nt + tile) * cut.nc * tru + (in >> 4)) * unit_floats(HDP);
+    constexpr size_t step = (size_t)tru * unit_floats(HDP);
+    float M = -INFINITY;
+    for (int i = lane; i < nc; i += kWave) M = fmaxf(M, u[i * step + (in & 15)]);
+    M = wave_max(M);
+    float L = 0.0f, o[VL] = {};
+    for (int i = 0; i < nc; ++i) {
+        const float w = state_weight(u[i * step + (in & 15)], M);
+        L += w * u[i * step + 16 + (in & 15)];
+#pragma unroll
+        for (int v = 0; v < VL; ++v) o[v] += w * u[i * step + 32 + (in & 15) * HDP + lane + 64 * v];
+    }
+    const Place pl = place(a, q, kvh, row);
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+#pragma unroll
+    for (int v = 0; v < VL; ++v)
+        if (lane + 64 * v < a.d.hd)
+            a.out[(size_t)pl.t * a.out_stride + (size_t)pl.h * a.d.hd + lane + 64 * v] = o[v] * inv;
+}
+// wide: whether the wide launch ran before.
+template <int HDP>
+__global__ __launch_bounds__(256) void attn_merge_kernel(AttnArgs a, int wide) {
+    const AttnHeader *hw = AttnWs<false>::header(a.ws), *ht = AttnWs<true>::header(a.ws);
+    const int nw = wide ? hw->merge_rows : 0, nt = a.thin ? ht->merge_rows : 0;
+    for (int id = blockIdx.x * 4 + (threadIdx.x >> 6); id < nw + nt; id += gridDim.x * 4)
+        if (id < nt)
+            merge_row<HDP, true>(a, ht, id);
+        else
+            merge_row<HDP, false>(a, hw, id - nt);
 }
 
 PagedDims dims_of(const rbt_paged_kv &kv) {
@@ -366,9 +1139,54 @@ hipError_t launch_paged_append(const Launch &L, const rbt_paged_kv &kv, const rb
                                    : launch(L, append_kernel<RBT_DT_F32>, g, dim3(256), 0, a);
 }
 
-hipError_t launch_paged_attn(const Launch &L, const rbt_paged_kv &kv, const rbt_paged_batch &b, const float *q,
-                             uint64_t q_stride, int T, int n_heads, float scale, int window, float *out,
-                             uint64_t out_stride) {
+namespace {
+// LDS past 64 KiB has to be asked for, once per kernel and device.
+template <typename F>
+hipError_t ask_lds(F kernel, int bytes, std::atomic<uint64_t> &asked) {
+    int dev = 0;
+    const hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return e;
+    const uint64_t bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
+    if (asked.load(std::memory_order_relaxed) & bit) return hipSuccess;
+    const hipError_t f = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (f == hipSuccess) asked.fetch_or(bit, std::memory_order_relaxed);
+    return f;
+}
+
+template <int DT, int HDP>
+hipError_t launch_attn(const Launch &L, const Launch &Lm, AttnArgs a) {
+    using W = WideShape<DT, HDP>;
+    const int G = a.n_heads / a.d.n_kv;
+    // Requests of up to 16 rows have a launch of their own on a bf16 cache, where its tiles and the step's prefix
+    // sums fit LDS (head dims above 128: up to 2900 requests). A launch that no request can belong to is left out;
+    // otherwise each finds its requests on the device.
+    a.thin = DT == RBT_DT_BF16 && G <= kThinRows && attn_lds(ThinShape<HDP>::TILE, a.n_req) <= kLdsBytes;
+    const bool wide = !a.thin || (int64_t)a.T * G > kThinRows;
+    static std::atomic<uint64_t> asked_w{0}, asked_t{0};
+    hipError_t e = hipSuccess;
+    if (wide) {
+        static_assert(attn_lds(W::TILE, kPagedMaxReq) <= kLdsBytes, "the wide launch takes any step");
+        e = ask_lds(attn_wide_kernel<DT, HDP>, attn_lds(W::TILE, kPagedMaxReq), asked_w);
+        if (e == hipSuccess)
+            e = launch(a.thin ? Lm : L, attn_wide_kernel<DT, HDP>, dim3(256 * W::PER_CU), dim3(256),
+                       (uint32_t)attn_lds(W::TILE, a.n_req), a);
+    }
+    if constexpr (DT == RBT_DT_BF16) {
+        using Th = ThinShape<HDP>;
+        if (a.thin && e == hipSuccess)
+            e = ask_lds(attn_thin_kernel<HDP>, std::min(attn_lds(Th::TILE, kPagedMaxReq), kLdsBytes), asked_t);
+        if (a.thin && e == hipSuccess)
+            e = launch(L, attn_thin_kernel<HDP>, dim3(256 * Th::PER_CU), dim3(256), (uint32_t)attn_lds(Th::TILE, a.n_req), a);
+    }
+    if (e != hipSuccess) return e;
+    return launch(Lm, attn_merge_kernel<HDP>, dim3(1024), dim3(256), 0, a, (int)wide);
+}
+}  // namespace
+
+hipError_t launch_paged_attn(const Launch &L, const Launch &Lm, const rbt_paged_kv &kv, const rbt_paged_batch &b,
+                             const float *q, uint64_t q_stride, int T, int n_heads, float scale, int window, float *out,
+                             uint64_t out_stride, void *ws) {
     if (T < 1 || b.n_req < 1) return hipSuccess;
     AttnArgs a;
     a.d = dims_of(kv);
@@ -377,7 +1195,7 @@ hipError_t launch_paged_attn(const Launch &L, const rbt_paged_kv &kv, const rbt_
     a.T = T;
     a.n_heads = n_heads;
     a.window = window;
-    a.scale = scale;
+    a.scale2 = scale * 1.44269504088896340736f;
     a.tables = b.tables;
     a.kv_len = b.kv_len;
     a.q_start = b.q_start;
@@ -387,6 +1205,18 @@ hipError_t launch_paged_attn(const Launch &L, const rbt_paged_kv &kv, const rbt_
     a.out = out;
     a.q_stride = q_stride;
     a.out_stride = out_stride;
+    a.ws = static_cast<uint8_t *>(ws);
+    const auto a16 = [](const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
+    const int esz = kv.dtype == RBT_DT_BF16 ? 2 : 4;
+    if (kv.head_dim % 8 == 0 && a16(q) && a16(out) && a16(kv.k) && a16(kv.v) && q_stride % 4 == 0 && out_stride % 4 == 0 &&
+        a.d.block_stride * esz % 16 == 0) {
+        const int hdp = kv.head_dim <= 64 ? 64 : kv.head_dim <= 128 ? 128 : 256;
+        if (kv.dtype == RBT_DT_BF16)
+            return hdp == 64 ? launch_attn<RBT_DT_BF16, 64>(L, Lm, a)
+                             : hdp == 128 ? launch_attn<RBT_DT_BF16, 128>(L, Lm, a) : launch_attn<RBT_DT_BF16, 256>(L, Lm, a);
+        return hdp == 64 ? launch_attn<RBT_DT_F32, 64>(L, Lm, a)
+                         : hdp == 128 ? launch_attn<RBT_DT_F32, 128>(L, Lm, a) : launch_attn<RBT_DT_F32, 256>(L, Lm, a);
+    }
     const uint64_t rows = (uint64_t)T * (uint64_t)n_heads;
     const dim3 g((unsigned)(rows < 65536 ? rows : 65536));
     return kv.dtype == RBT_DT_BF16 ? launch(L, attn_any_kernel<RBT_DT_BF16>, g, dim3(256), 0, a)

@@ -399,10 +399,10 @@ hipError_t launch_record_routing(const Launch &L, const StepState *st, const int
 // Lr: launch context of the rows' own launch, which large steps take.
 hipError_t launch_paged_plan(const Launch &L, const Launch &Lr, const rbt_paged_plan &p);
 hipError_t launch_paged_append(const Launch &L, const rbt_paged_kv &kv, const rbt_paged_rows &w);
-// Strides and scale as given to the kernels (not 0).
-hipError_t launch_paged_attn(const Launch &L, const rbt_paged_kv &kv, const rbt_paged_batch &b, const float *q,
-                             uint64_t q_stride, int T, int n_heads, float scale, int window, float *out,
-                             uint64_t out_stride);
+// Strides and scale as given to the kernels (not 0). Lm: launch context of the merge. ws: kPagedWsBytes.
+hipError_t launch_paged_attn(const Launch &L, const Launch &Lm, const rbt_paged_kv &kv, const rbt_paged_batch &b,
+                             const float *q, uint64_t q_stride, int T, int n_heads, float scale, int window, float *out,
+                             uint64_t out_stride, void *ws);
 
 // Dense matvec (one row per wave).
 hipError_t launch_matvec(const Launch &L, int dtype, const void *W, const float *x, float *out, int rows, int cols);
