@@ -1712,7 +1712,14 @@ int paged_ws_reserve(rbt_hip *h) {
     HIP_OK(h, hipStreamIsCapturing(h->stream, &cap));
     if (cap != hipStreamCaptureStatusNone)
         return fail(h, "paged_attn: the stream is being captured before rbt_hip_paged_reserve");
-    HIP_OK(h, hipMalloc(&h->paged_ws, kPagedWsBytes));
+    void *ws = nullptr;
+    HIP_OK(h, hipMalloc(&ws, kPagedWsBytes));
+    const hipError_t e = HIP_TRY(hipMemsetAsync(ws, 0, kPagedWsBytes, h->stream));  // its item counters
+    if (e != hipSuccess) {
+        (void)hipFree(ws);
+        return fail(h, "paged_reserve: %s failed: %s", failed_call(), hipGetErrorString(e));
+    }
+    h->paged_ws = ws;
     return 1;
 }
 

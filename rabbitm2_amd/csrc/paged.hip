@@ -6,6 +6,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "paged.h"
 #include "rbt2_internal.h"
@@ -376,6 +377,7 @@ static_assert(kMaxChunk % 128 == 0, "whole tiles");
 // o [16][HDP].
 struct AttnHeader {
     int32_t chunk, merge_rows, pad[2];
+    int32_t taken[8][16];  // items that each XCD's blocks took beyond their first, a line each; 0 between the calls
     int32_t merge[kPagedMaxReq + 4], units[kPagedMaxReq + 4];
 };
 constexpr size_t kWsThin = kPagedWsBytes / 4;  // of it, with its header
@@ -406,6 +408,16 @@ __device__ __forceinline__ Cut cut_of(const AttnArgs &a, const Request &q, int c
     const int span = a.window > 0 ? min(q.n, min(a.window, q.n) + (tr - 1) / G + 1) : q.n;
     c.nc = max(1, (int)(((long long)span + chunk - 1) / chunk));
     return c;
+}
+
+// The n pieces of len positions that a tile of span positions is cut into: equal up to whole tiles, none empty (len <=
+// chunk, both multiples of 128).
+struct Pieces {
+    int n, len;
+};
+__device__ __forceinline__ Pieces pieces_of(int span, int chunk) {
+    const int n = max(1, (int)(((long long)span + chunk - 1) / chunk));
+    return {n, (int)(((long long)span + n - 1) / n + 127) / 128 * 128};
 }
 
 // Sum over the block's 256 threads and this thread's exclusive prefix.
@@ -522,10 +534,39 @@ __device__ __forceinline__ float group_sum(float v) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// LDS layout of a tile part: rows of HDP bf16 and 16 bytes more, so that the same chunk of 16 rows (a K operand) and
-// the same 32 bytes of 16 rows (V^T) lie in all banks evenly, at fixed distances from a lane's first.
+// LDS layouts of a tile part, in which the same 16-byte chunk of 16 rows (a K operand) and the same 32 bytes of 16
+// rows (V^T) lie in all banks evenly. k_at(t, st) and v_at(t, d): a lane's byte of the operands of key group t, k-step
+// st and of dims 16 d.
+// Rows of HDP bf16 and 16 bytes more: every operand at a fixed distance from a lane's first.
 template <int HDP>
-constexpr int kTileRow = HDP * 2 + 16;
+struct PaddedTile {
+    static constexpr int ROW = HDP * 2 + 16;
+    int k0, v0;
+    __device__ __forceinline__ PaddedTile() {
+        const int c = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
+        k0 = c * ROW + 16 * g;
+        v0 = (4 * g + (c >> 2)) * ROW + 8 * (c & 3);
+    }
+    __device__ __forceinline__ int k_at(int t, int st) const { return k0 + t * 16 * ROW + st * 64; }
+    __device__ __forceinline__ int v_at(int t, int d) const { return v0 + t * 16 * ROW + d * 32; }
+};
+// Rows of HDP bf16 whose chunks are permuted by the row (chunk ^ key(row)): what direct copies can write, whose lanes
+// each choose what they read but not where it lands.
+template <int HDP>
+struct SwizzledTile {
+    static constexpr int ROW = HDP * 2, CH = HDP / 8, KN = CH < 16 ? CH / 4 : 4, VN = CH < 16 ? CH / 2 : 8;
+    __device__ static __forceinline__ int key(int row) { return CH == 8 ? (row >> 1) & 7 : row & 15; }
+    int k[KN], v[VN];
+    __device__ __forceinline__ SwizzledTile() {
+        const int c = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4, vr = 4 * g + (c >> 2);
+#pragma unroll
+        for (int i = 0; i < KN; ++i) k[i] = c * ROW + ((4 * i + g) ^ key(c)) * 16;
+#pragma unroll
+        for (int i = 0; i < VN; ++i) v[i] = vr * ROW + ((2 * i + ((c & 3) >> 1)) ^ key(vr)) * 16 + 8 * (c & 1);
+    }
+    __device__ __forceinline__ int k_at(int t, int st) const { return k[st % KN] + t * 16 * ROW + st / KN * 64 * KN; }
+    __device__ __forceinline__ int v_at(int t, int d) const { return v[d % VN] + t * 16 * ROW + d / VN * 32 * VN; }
+};
 
 extern __shared__ __align__(16) uint8_t smem[];
 
@@ -538,15 +579,11 @@ struct WaveState {
     int pos[NQ];  // this lane's query's position
 };
 
-// 32 positions, rows row0 .. row0 + 31 of the staged tile (keys at byte k_off of LDS, values at v_off, parts
-// `part` bytes apart); seen(n): bit 4 t + i, whether query n of this lane sees key 16 t + 4 g + i of them
+// 32 positions, staged from byte k_off (keys) and v_off (values) of LDS on, parts `part` bytes apart; seen(n): bit 4 t + i, whether query n of this lane sees key 16 t + 4 g + i of them
 // (asked where !full).
-template <int HDP, int NQ, int NP, int part, typename Seen>
-__device__ __forceinline__ void attn_step(WaveState<HDP, NQ> &w, int k_off, int v_off, int row0, float scale2,
+template <int HDP, int NQ, int NP, int part, typename Tile, typename Seen>
+__device__ __forceinline__ void attn_step(WaveState<HDP, NQ> &w, const Tile &tile, int k_off, int v_off, float scale2,
                                           bool full, Seen seen) {
-    constexpr int RS = kTileRow<HDP>;
-    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-    const int k_at = k_off + (row0 + c) * RS + 16 * g, v_at = v_off + (row0 + 4 * g + (c >> 2)) * RS + 8 * (c & 3);
     f32x4 s[NQ][2];
 #pragma unroll
     for (int n = 0; n < NQ; ++n) s[n][0] = s[n][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -557,7 +594,7 @@ __device__ __forceinline__ void attn_step(WaveState<HDP, NQ> &w, int k_off, int 
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int kp = 0; kp < NP; ++kp) {
-                const u32x4 k = *reinterpret_cast<const u32x4 *>(smem + k_at + kp * part + t * 16 * RS + st * 64);
+                const u32x4 k = *reinterpret_cast<const u32x4 *>(smem + (k_off + kp * part) + tile.k_at(t, st));
 #pragma unroll
                 for (int qp = 0; qp + kp < 3; ++qp)
 #pragma unroll
@@ -623,7 +660,7 @@ __device__ __forceinline__ void attn_step(WaveState<HDP, NQ> &w, int k_off, int 
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 const u32x2 h = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (__attribute__((address_space(3))) s16x4 *)(smem + v_at + vp * part + t * 16 * RS + d * 32)));
+                    (__attribute__((address_space(3))) s16x4 *)(smem + (v_off + vp * part) + tile.v_at(t, d))));
                 v[2 * t] = h[0];
                 v[2 * t + 1] = h[1];
             }
@@ -708,15 +745,37 @@ struct Stage {
         }
     }
     __device__ __forceinline__ void store(int k_off, int v_off, int part, int tid) {
-        const int at = tid / CH * kTileRow<HDP> + 16 * (tid % CH);
+        const int at = tid / CH * PaddedTile<HDP>::ROW + 16 * (tid % CH);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int off = at + i * ROWS * kTileRow<HDP>;
+            const int off = at + i * ROWS * PaddedTile<HDP>::ROW;
             put(k[i], k_off + off, part);
             put(v[i], v_off + off, part);
         }
     }
 };
+
+// The same for a bf16 tile of a block's four waves as direct copies into LDS (SwizzledTile), not waited for. A head
+// dim below HDP: the chunks behind it repeat its last (the query's are 0, and the output's are not stored).
+template <int HDP, int KEYS>
+__device__ __forceinline__ void copy_tile(const AttnArgs &a, const int32_t *s_tab, int page0, int kvh, int j, int last,
+                                          int buf) {
+    using Tile = SwizzledTile<HDP>;
+    constexpr int ROWS = 64 / Tile::CH, N = KEYS / 4 / ROWS;  // rows per copy, copies per wave (of K, of V)
+    static_assert(N * 4 * ROWS == KEYS, "whole copies");
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)smem + (uint32_t)buf;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int row0 = (wv * N + i) * ROWS, row = row0 + lane / Tile::CH;
+        const int chunk = min((lane % Tile::CH) ^ Tile::key(row), a.d.hd / 8 - 1);
+        const int pos = min(j + row, last), page = (int)page_of((uint32_t)pos, a.d.div);
+        const int b = max(s_tab[page - page0], 0);
+        const uint64_t at = (paged_row(a.d, b, kvh, pos - page * a.d.block_size) + 8 * chunk) * 2;
+        lds_dma16(static_cast<const uint8_t *>(a.kc) + at, lds + (uint32_t)(row0 * Tile::ROW));
+        lds_dma16(static_cast<const uint8_t *>(a.vc) + at, lds + (uint32_t)((KEYS + row0) * Tile::ROW));
+    }
+}
 
 // A row's place: its token and head.
 struct Place {
@@ -731,8 +790,9 @@ __device__ __forceinline__ Place place(const AttnArgs &a, const Request &q, int 
 struct Item {
     Request q;
     Cut cut;
-    int r, kvh, row0, n_rows, pa, pb, k0, k1;  // rows row0 .. row0 + n_rows - 1 at positions pa .. pb; chunk [k0, k1)
-    float *unit;                               // its partials
+    int r, kvh, row0, n_rows, pa, pb, k0, k1;  // rows row0 .. row0 + n_rows - 1 at positions pa .. pb; piece [k0, k1)
+    bool live, split;                          // whether the tile has this piece, and more than one
+    float *unit;                               // the piece's partials
 };
 template <bool THIN, int HDP>
 __device__ __forceinline__ Item item_of(const AttnArgs &a, int it, int chunk, const int32_t *s_items,
@@ -744,32 +804,52 @@ __device__ __forceinline__ Item item_of(const AttnArgs &a, int it, int chunk, co
     x.q = request(a, x.r);
     x.cut = cut_of<THIN>(a, x.q, chunk);
     int local = it - __builtin_amdgcn_readfirstlane(s_items[x.r]);
-    const int c = local % x.cut.nc;
-    local /= x.cut.nc;
-    x.kvh = local / x.cut.nt;
-    const int tile = x.cut.nt - 1 - local % x.cut.nt;  // the longest tiles first
+    // with a multiple of eight heads each eighth of the items has its own; the longest tiles first, their pieces and
+    // heads together
+    const int hx = a.d.n_kv % 8 == 0 ? a.d.n_kv / 8 : a.d.n_kv, per_group = x.cut.nt * x.cut.nc * hx;
+    const int group = local / per_group;
+    local -= group * per_group;
+    const int tile = x.cut.nt - 1 - local / (x.cut.nc * hx);
+    local %= x.cut.nc * hx;
+    const int c = local / hx;
+    x.kvh = group * hx + local % hx;
     x.row0 = tile * tr;
     x.n_rows = min(tr, x.cut.rows - x.row0);
     x.pa = place(a, x.q, x.kvh, x.row0).pos;
     x.pb = place(a, x.q, x.kvh, x.row0 + x.n_rows - 1).pos;
     const int lo = a.window > 0 ? max(0, x.pa - a.window + 1) : 0;
-    x.k0 = (int)min((long long)lo + (long long)c * chunk, (long long)kPagedMaxLen);
-    x.k1 = min(x.pb + 1, (int)min((long long)x.k0 + chunk, (long long)kPagedMaxLen));
+    const Pieces pc = pieces_of(max(x.pb + 1 - lo, 0), chunk);
+    x.live = c < pc.n;
+    x.k0 = x.live ? lo + c * pc.len : 0;
+    x.k1 = x.live ? min(x.pb + 1, x.k0 + min(pc.len, x.pb + 1 - x.k0)) : 0;
+    x.split = pc.n > 1;
     x.unit = AttnWs<THIN>::partials(a.ws) +
              ((size_t)__builtin_amdgcn_readfirstlane(s_units[x.r]) +
               ((size_t)(x.kvh * x.cut.nt + tile) * x.cut.nc + c) * (tr / 16)) * unit_floats(HDP);
     return x;
 }
-// Items in order of (request, head, tile, chunk); an eighth of them to each XCD (blocks b % 8), so that a head's row
-// tiles read its keys and values through one L2.
-struct ItemRange {
-    int first, end, step;
+// An eighth of the items to each XCD (blocks b % 8), so that a head's row tiles read its keys and values through one
+// L2. A block starts with the item of its own number and then takes the next one left of its eighth: taken() is asked
+// for early, its answer used by next() at the item's end.
+struct ItemQueue {
+    int it, end, base;
+    int32_t *taken;
+    __device__ __forceinline__ ItemQueue(int n_items, AttnHeader *hdr) {
+        const int xcd = blockIdx.x & 7, i0 = (int)((long long)n_items * xcd / 8);
+        end = (int)((long long)n_items * (xcd + 1) / 8);
+        it = i0 + (int)(blockIdx.x >> 3);
+        base = i0 + (int)(gridDim.x >> 3);
+        taken = &hdr->taken[xcd][0];
+    }
+    __device__ __forceinline__ int ask() const { return threadIdx.x == 0 ? atomicAdd(taken, 1) : 0; }
+    // for all threads, with a barrier after and before every other use of the shared word
+    __device__ __forceinline__ void next(int ticket, int *s_next) {
+        if (threadIdx.x == 0) *s_next = ticket;
+        __syncthreads();
+        it = base + __builtin_amdgcn_readfirstlane(*s_next);
+        __syncthreads();
+    }
 };
-__device__ __forceinline__ ItemRange item_range(int n_items) {
-    const int xcd = blockIdx.x & 7;
-    const int i0 = (int)((long long)n_items * xcd / 8), i1 = (int)((long long)n_items * (xcd + 1) / 8);
-    return {i0 + (int)(blockIdx.x >> 3), i1, (int)(gridDim.x >> 3)};
-}
 
 // Block numbers of the pages that positions j0 .. j1 - 1 (at most tab_span of them) lie on, into s_tab; -1 for one
 // outside the cache: whether there is any. For all threads of the block.
@@ -818,7 +898,7 @@ __device__ __forceinline__ void again_rows(const AttnArgs &a, const Item &x, con
         const int j0 = a.window > 0 ? max(x.k0, pl.pos - a.window + 1) : x.k0;
         float m, l, o;
         row_any<DT>(a, *reinterpret_cast<RowShared *>(smem), x.r, pl.t, pl.h, j0, min(x.k1, pl.pos + 1), &m, &l, &o);
-        if (x.cut.nc > 1) {
+        if (x.split) {
             float *un = x.unit + (size_t)(row >> 4) * unit_floats(HDP);
             if (threadIdx.x == 0) {
                 un[row & 15] = m;
@@ -838,7 +918,7 @@ constexpr int attn_lds(int tile, int n_req) { return tile + kTabBytes + 8 * (n_r
 // Requests of up to 16 rows.
 template <int HDP>
 struct ThinShape {
-    static constexpr int WAVE = 2 * 32 * kTileRow<HDP>;  // a wave's own keys and values, and later its rows
+    static constexpr int WAVE = 2 * 32 * PaddedTile<HDP>::ROW;  // a wave's own keys and values, and later its rows
     static constexpr int TILE = 4 * WAVE;
     static constexpr int PER_CU = HDP <= 128 ? 2 : 1;  // blocks that share a CU
     static_assert(kThinRows * (HDP + 4) * 4 <= WAVE, "a wave's rows fit its tile");
@@ -849,19 +929,25 @@ __global__ __launch_bounds__(256, (ThinShape<HDP>::PER_CU)) void attn_thin_kerne
     constexpr int DT = RBT_DT_BF16, WAVE = ThinShape<HDP>::WAVE;
     __shared__ long long s_w[4];
     __shared__ float s_m[4][kThinRows], s_l[4][kThinRows];
-    __shared__ int s_flag[kThinRows];
+    __shared__ int s_flag[kThinRows], s_next;
     int32_t *s_tab = reinterpret_cast<int32_t *>(smem + ThinShape<HDP>::TILE), *s_items = s_tab + kTabPages,
             *s_units = s_items + a.n_req + 1;
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
     const int chunk = __builtin_amdgcn_readfirstlane(
         schedule<true>(a, AttnWs<true>::max_units(HDP), s_items, s_units, s_w));
-    const ItemRange items = item_range(__builtin_amdgcn_readfirstlane(s_items[a.n_req]));
+    ItemQueue items(__builtin_amdgcn_readfirstlane(s_items[a.n_req]), AttnWs<true>::header(a.ws));
     const int span = tab_span(a);
-    for (int it = items.first; it < items.end; it += items.step) {
-        const Item x = item_of<true, HDP>(a, it, chunk, s_items, s_units);
+    const PaddedTile<HDP> tl;
+    while (items.it < items.end) {
+        const Item x = item_of<true, HDP>(a, items.it, chunk, s_items, s_units);
+        const int ticket = items.ask();
+        if (!x.live) {
+            items.next(ticket, &s_next);
+            continue;
+        }
         WaveState<HDP, 1> w;
         wave_init<HDP, 1>(w, a, x.q, x.cut.rows, x.kvh, x.row0);
-        const int k_off = wv * WAVE, v_off = k_off + 32 * kTileRow<HDP>;
+        const int k_off = wv * WAVE, v_off = k_off + 32 * PaddedTile<HDP>::ROW;
         for (int w0 = x.k0; w0 < x.k1; w0 += span) {
             const int w1 = min(x.k1, w0 + min(span, x.k1 - w0)), page0 = (int)page_of((uint32_t)w0, a.d.div);
             const bool bad = fill_tab(a, x.r, w0, w1, s_tab);
@@ -874,12 +960,11 @@ __global__ __launch_bounds__(256, (ThinShape<HDP>::PER_CU)) void attn_thin_kerne
                 __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
                 if (j + 128 < w1) st.load(a, s_tab, page0, x.kvh, j + 128, w1 - 1, lane);
                 const bool full = !bad && j + 32 <= min(w1, x.pa + 1) && (a.window <= 0 || j > x.pb - a.window);
-                attn_step<HDP, 1, 1, 0>(w, k_off, v_off, 0, a.scale2, full,
+                attn_step<HDP, 1, 1, 0>(w, tl, k_off, v_off, a.scale2, full,
                                         [&](int n) { return seen_bits(a, j, w1, w.pos[n], s_tab, page0, bad); });
             }
         }
         // the four waves' states, joined; each wave's rows lie where its tile was
-        const bool split = x.cut.nc > 1;
         w.l[0] = group_sum(w.l[0]);
         if (g == 0) {
             s_m[wv][c] = w.m[0];
@@ -914,7 +999,7 @@ __global__ __launch_bounds__(256, (ThinShape<HDP>::PER_CU)) void attn_thin_kerne
         if (row < x.n_rows) {
             if (again) {
                 if (y == 0) s_flag[row] = 1;
-            } else if (split) {
+            } else if (x.split) {
                 if (y == 0) {
                     x.unit[row] = M;
                     x.unit[16 + row] = L;
@@ -932,7 +1017,7 @@ __global__ __launch_bounds__(256, (ThinShape<HDP>::PER_CU)) void attn_thin_kerne
             }
         }
         if (__syncthreads_or(again && row < x.n_rows)) again_rows<DT, HDP>(a, x, s_flag);
-        __syncthreads();
+        items.next(ticket, &s_next);
     }
 }
 
@@ -941,8 +1026,11 @@ template <int DT, int HDP>
 struct WideShape {
     static constexpr int NP = DT == RBT_DT_BF16 ? 1 : 3;
     static constexpr int KEYS = DT == RBT_DT_BF16 && HDP <= 128 ? 64 : 32;
-    static constexpr int PART = KEYS * kTileRow<HDP>;
-    static constexpr int TILE = 2 * NP * PART;
+    // bf16: two buffers that direct copies fill in turn; f32: one of parts, through registers
+    static constexpr bool COPY = DT == RBT_DT_BF16;
+    using Tile = std::conditional_t<COPY, SwizzledTile<HDP>, PaddedTile<HDP>>;
+    static constexpr int PART = KEYS * Tile::ROW, BUF = 2 * NP * PART;
+    static constexpr int TILE = COPY ? 2 * BUF : BUF;
     static constexpr int PER_CU = HDP <= 128 ? 2 : 1;
     static_assert(sizeof(RowShared) <= (size_t)TILE, "row_any's LDS");
 };
@@ -950,45 +1038,66 @@ template <int DT, int HDP>
 __global__ __launch_bounds__(256, (WideShape<DT, HDP>::PER_CU)) void attn_wide_kernel(AttnArgs a) {
     using Sh = WideShape<DT, HDP>;
     __shared__ long long s_w[4];
-    __shared__ int s_flag[kWideRows];
+    __shared__ int s_flag[kWideRows], s_next;
     int32_t *s_tab = reinterpret_cast<int32_t *>(smem + Sh::TILE), *s_items = s_tab + kTabPages,
             *s_units = s_items + a.n_req + 1;
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
     const int chunk = __builtin_amdgcn_readfirstlane(
         schedule<false>(a, AttnWs<false>::max_units(HDP), s_items, s_units, s_w));
-    const ItemRange items = item_range(__builtin_amdgcn_readfirstlane(s_items[a.n_req]));
+    ItemQueue items(__builtin_amdgcn_readfirstlane(s_items[a.n_req]), AttnWs<false>::header(a.ws));
     const int span = tab_span(a);
-    for (int it = items.first; it < items.end; it += items.step) {
-        const Item x = item_of<false, HDP>(a, it, chunk, s_items, s_units);
-        if (x.k0 >= x.k1 && x.k0 > 0) continue;  // a chunk behind the tile's positions: the merge knows
+    const typename Sh::Tile tl;
+    while (items.it < items.end) {
+        const Item x = item_of<false, HDP>(a, items.it, chunk, s_items, s_units);
+        const int ticket = items.ask();
+        if (!x.live) {
+            items.next(ticket, &s_next);
+            continue;
+        }
         const int wr0 = x.row0 + 32 * wv;
         const bool active = 32 * wv < x.n_rows;
         const int wa = place(a, x.q, x.kvh, min(wr0, x.cut.rows - 1)).pos,
                   wb = place(a, x.q, x.kvh, min(wr0 + 31, x.cut.rows - 1)).pos;
         WaveState<HDP, 2> w;
         wave_init<HDP, 2>(w, a, x.q, x.cut.rows, x.kvh, wr0);
-        constexpr int k_off = 0, v_off = Sh::NP * Sh::PART;
         for (int w0 = x.k0; w0 < x.k1; w0 += span) {
             const int w1 = min(x.k1, w0 + min(span, x.k1 - w0)), page0 = (int)page_of((uint32_t)w0, a.d.div);
             const bool bad = fill_tab(a, x.r, w0, w1, s_tab);
-            Stage<DT, HDP, Sh::KEYS, 256> st;
-            st.load(a, s_tab, page0, x.kvh, w0, w1 - 1, tid);
-            for (int jt = w0; jt < w1; jt += Sh::KEYS) {
-                __syncthreads();
-                st.store(k_off, v_off, Sh::PART, tid);
-                __syncthreads();
-                if (jt + Sh::KEYS < w1) st.load(a, s_tab, page0, x.kvh, jt + Sh::KEYS, w1 - 1, tid);
+            // the wave's part of a staged tile from position jt on
+            auto steps = [&](int jt, int buf) {
                 for (int u = 0; u < Sh::KEYS; u += 32) {
                     const int j = jt + u;
                     if (!active || j >= w1 || j > wb || (a.window > 0 && j + 31 <= wa - a.window)) continue;
                     const bool full = !bad && j + 32 <= min(w1, wa + 1) && (a.window <= 0 || j > wb - a.window);
+                    const int k_off = buf + u * Sh::Tile::ROW;
                     attn_step<HDP, 2, Sh::NP, Sh::PART>(
-                        w, k_off, v_off, u, a.scale2, full,
+                        w, tl, k_off, k_off + Sh::NP * Sh::PART, a.scale2, full,
                         [&](int n) { return seen_bits(a, j, w1, w.pos[n], s_tab, page0, bad); });
+                }
+            };
+            if constexpr (Sh::COPY) {
+                copy_tile<HDP, Sh::KEYS>(a, s_tab, page0, x.kvh, w0, w1 - 1, 0);
+                int buf = 0;
+                for (int jt = w0; jt < w1; jt += Sh::KEYS) {
+                    wait_dma<0>();
+                    __syncthreads();  // this tile has landed for all, and the last one has been read
+                    if (jt + Sh::KEYS < w1)
+                        copy_tile<HDP, Sh::KEYS>(a, s_tab, page0, x.kvh, jt + Sh::KEYS, w1 - 1, buf ^ Sh::BUF);
+                    steps(jt, buf);
+                    buf ^= Sh::BUF;
+                }
+            } else {
+                Stage<DT, HDP, Sh::KEYS, 256> st;
+                st.load(a, s_tab, page0, x.kvh, w0, w1 - 1, tid);
+                for (int jt = w0; jt < w1; jt += Sh::KEYS) {
+                    __syncthreads();
+                    st.store(0, Sh::NP * Sh::PART, Sh::PART, tid);
+                    __syncthreads();
+                    if (jt + Sh::KEYS < w1) st.load(a, s_tab, page0, x.kvh, jt + Sh::KEYS, w1 - 1, tid);
+                    steps(jt, 0);
                 }
             }
         }
-        const bool split = x.cut.nc > 1;
         if (tid < kWideRows) s_flag[tid] = 0;
         __syncthreads();
         bool any = false;
@@ -1005,7 +1114,7 @@ __global__ __launch_bounds__(256, (WideShape<DT, HDP>::PER_CU)) void attn_wide_k
             if (again) {
                 s_flag[row] = 1;
                 any = true;
-            } else if (split) {
+            } else if (x.split) {
                 float *un = x.unit + (size_t)(row >> 4) * unit_floats(HDP);
                 if (g == 0) {
                     un[c] = w.m[n];
@@ -1024,7 +1133,7 @@ __global__ __launch_bounds__(256, (WideShape<DT, HDP>::PER_CU)) void attn_wide_k
             }
         }
         if (__syncthreads_or(any)) again_rows<DT, HDP>(a, x, s_flag);
-        __syncthreads();
+        items.next(ticket, &s_next);
     }
 }
 
@@ -1039,7 +1148,8 @@ __device__ __forceinline__ void merge_row(const AttnArgs &a, const AttnHeader *h
     const int row0 = tile * tr, n_rows = min(tr, cut.rows - row0), in = row - row0;
     const int pa = place(a, q, kvh, row0).pos, pb = place(a, q, kvh, row0 + n_rows - 1).pos;
     const int lo = a.window > 0 ? max(0, pa - a.window + 1) : 0;
-    const int nc = max(1, min(cut.nc, (int)(((long long)pb + 1 - lo + chunk - 1) / chunk)));  // those that hold positions
+    const int nc = pieces_of(max(pb + 1 - lo, 0), chunk).n;
+    if (nc == 1) return;  // a tile of a cut request that is not cut itself: written by its block
     const float *u = AttnWs<THIN>::partials(a.ws) +
                      ((size_t)hdr->units[r] + (size_t)(kvh * cut.nt + tile) * cut.nc * tru + (in >> 4)) * unit_floats(HDP);
     constexpr size_t step = (size_t)tru * unit_floats(HDP);
@@ -1063,7 +1173,8 @@ __device__ __forceinline__ void merge_row(const AttnArgs &a, const AttnHeader *h
 // wide: whether the wide launch ran before.
 template <int HDP>
 __global__ __launch_bounds__(256) void attn_merge_kernel(AttnArgs a, int wide) {
-    const AttnHeader *hw = AttnWs<false>::header(a.ws), *ht = AttnWs<true>::header(a.ws);
+    AttnHeader *hw = AttnWs<false>::header(a.ws), *ht = AttnWs<true>::header(a.ws);
+    if (blockIdx.x == 0 && threadIdx.x < 8) hw->taken[threadIdx.x][0] = ht->taken[threadIdx.x][0] = 0;
     const int nw = wide ? hw->merge_rows : 0, nt = a.thin ? ht->merge_rows : 0;
     for (int id = blockIdx.x * 4 + (threadIdx.x >> 6); id < nw + nt; id += gridDim.x * 4)
         if (id < nt)

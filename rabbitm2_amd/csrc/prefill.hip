@@ -375,21 +375,9 @@ __global__ __launch_bounds__(256) void split_hilo_kernel(const float *__restrict
 }
 
 // ---------------------------------------------------------------- grouped GEMM
-// Direct HBM -> LDS copies (global_load_lds_dwordx4): each lane's 16 bytes land at LDS m0 + 16*lane, so
-// one instruction fills 1 KiB of LDS in lane order and costs no registers. They are issued from inline
-// assembly and waited for by hand (s_waitcnt vmcnt): the compiler, which would otherwise wait for every
-// pending copy before any LDS read, does not see them. The main loop issues no other vector-memory
-// operation, so vmcnt counts exactly these copies.
-__device__ __forceinline__ void lds_dma16(const void *g, uint32_t lds_byte) {
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds_byte), "v"(g) : "memory", "m0");
-}
-// The same for data read once (expert weights): a streaming (non-temporal) load.
+// lds_dma16 for data read once (expert weights): a streaming (non-temporal) load.
 __device__ __forceinline__ void lds_dma16_stream(const void *g, uint32_t lds_byte) {
     asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(lds_byte), "v"(g) : "memory", "m0");
-}
-template <int N>
-__device__ __forceinline__ void wait_dma() {
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 // Until at most `ahead` stages of n copies each (n = WI .. WI + AI, this wave's copies per stage) are
 // outstanding; copies complete in issue order. Both arguments are wave-uniform.

@@ -108,6 +108,19 @@ __device__ __forceinline__ void tile_of(int tau, const int32_t *__restrict__ m_o
     *e_out = e;
 }
 
+// Direct HBM -> LDS copies (global_load_lds_dwordx4): each lane's 16 bytes land at LDS m0 + 16*lane, so
+// one instruction fills 1 KiB of LDS in lane order and costs no registers. They are issued from inline
+// assembly and waited for by hand (s_waitcnt vmcnt): the compiler, which would otherwise wait for every
+// pending copy before any LDS read, does not see them. A loop that counts them issues no other
+// vector-memory operation, so vmcnt counts exactly these copies.
+__device__ __forceinline__ void lds_dma16(const void *g, uint32_t lds_byte) {
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds_byte), "v"(g) : "memory", "m0");
+}
+template <int N>
+__device__ __forceinline__ void wait_dma() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
 // Cross-lane moves through DPP (a VALU operand modifier, no LDS round trip). Within each row of 16
 // lanes: swap neighbours, swap pairs, mirror each half-row, mirror the row -- after four steps every
 // lane of a row holds the same row total (each step adds commutative partners, so all lanes of a
