@@ -372,11 +372,11 @@ constexpr int kTabPages = 1024;  // block numbers of a chunk held in LDS
 constexpr int kMinChunk = 128, kMaxChunk = kPagedMaxLen;  // positions, multiples of 128
 static_assert(kMaxChunk % 128 == 0, "whole tiles");
 
-// Workspace: for the wide and the thin launch each a header (chunk length, rows to merge) and the prefix sums of the
-// merge rows and of the partial units over the requests, then their partials: units of 16 rows, m [16], l [16],
+// Workspace: for the wide and the thin launch each a header (chunk length, blocks of merging) and the prefix sums of
+// those and of the partial units over the requests, then their partials: units of 16 rows, m [16], l [16],
 // o [16][HDP].
 struct AttnHeader {
-    int32_t chunk, merge_rows, pad[2];
+    int32_t chunk, merge_blocks, pad[2];
     int32_t taken[8][16];  // items that each XCD's blocks took beyond their first, a line each; 0 between the calls
     int32_t merge[kPagedMaxReq + 4], units[kPagedMaxReq + 4];
 };
@@ -420,88 +420,122 @@ __device__ __forceinline__ Pieces pieces_of(int span, int chunk) {
     return {n, (int)(((long long)span + n - 1) / n + 127) / 128 * 128};
 }
 
-// Sum over the block's 256 threads and this thread's exclusive prefix.
-__device__ __forceinline__ long long block_scan(long long v, long long *total, long long *s_w) {
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-    long long inc = v;
-    for (int off = 1; off < kWave; off <<= 1) {
-        const long long up = __shfl_up(inc, off, kWave);
-        if (lane >= off) inc += up;
-    }
-    __syncthreads();
-    if (lane == kWave - 1) s_w[wv] = inc;
-    __syncthreads();
-    long long before = 0;
-    for (int w = 0; w < wv; ++w) before += s_w[w];
-    *total = (s_w[0] + s_w[1]) + (s_w[2] + s_w[3]);
-    return before + inc - v;
+// Rows that a block of the merge launch joins: a few per wave, or where many pieces have to be read, as many as one
+// wave takes, the pieces dealt to the block's four.
+constexpr int kMergeManyPieces = 16;
+template <int HDP>
+__device__ __forceinline__ int merge_rows(int nc) { return 256 / HDP * (nc >= kMergeManyPieces ? 1 : 4); }
+
+// Inclusive prefix sum over the wave, by DPP: within rows of 16 lanes, then the rows' totals handed on.
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr:1
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
+    return v;
 }
 
-// A launch's items (request, head, row tile, chunk), by every block for itself: prefix sums over the requests into
+// A launch's items (request, head, row tile, piece), by every block for itself: prefix sums over the requests into
 // s_items [n_req + 1] and s_units. The chunk length spreads the work over about two rounds of blocks; it doubles
-// until the partials fit, which ends at the latest at kMaxChunk, where no tile is cut.
-template <bool THIN>
-__device__ int schedule(const AttnArgs &a, int units_max, int32_t *s_items, int32_t *s_units,
-                        long long *s_w) {
+// until the partials fit, which ends at the latest at kMaxChunk, where no tile is cut. Returns 0 where the launch has
+// no request.
+struct ScheduleShared {
+    float work[4];
+    int any[4], sum[4][3];
+};
+template <bool THIN, int HDP>
+__device__ int schedule(const AttnArgs &a, int32_t *s_items, int32_t *s_units, ScheduleShared &s) {
+    constexpr int tr = kTileRows<THIN>, kUnits = AttnWs<THIN>::max_units(HDP);
     const int per = (a.n_req + 255) / 256, r0 = min(a.n_req, (int)threadIdx.x * per), r1 = min(a.n_req, r0 + per);
-    long long work = 0, total;
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    AttnHeader *hdr = blockIdx.x == 0 ? AttnWs<THIN>::header(a.ws) : nullptr;  // one block tells the merge launch
+    // the first request of a thread (all of them, up to 256 requests) stays in registers
+    Request first{};
+    if (r0 < r1) first = request(a, r0);
+    auto req = [&](int r) { return r == r0 ? first : request(a, r); };
+    float work = 0.0f;
+    bool any = false;
     for (int r = r0; r < r1; ++r) {
-        const Request q = request(a, r);
+        const Request q = req(r);
         if (!q.m) continue;
         const Cut c = cut_of<THIN>(a, q, kMaxChunk);
-        work += (long long)c.nt * (a.window > 0 ? min(q.n, min(a.window, q.n) + kTileRows<THIN>) : q.n - q.m / 2);
+        any |= c.nt > 0;
+        work += (float)c.nt * (float)(a.window > 0 ? min(q.n, min(a.window, q.n) + tr) : q.n - q.m / 2);
     }
-    block_scan(work, &total, s_w);
-    long long chunk = (total * a.d.n_kv / (2 * gridDim.x) + 127) / 128 * 128;
-    chunk = min(max(chunk, (long long)kMinChunk), (long long)kMaxChunk);
+    work = wave_sum(work);
+    const bool wave_any = __any(any);
+    if (lane == 0) {
+        s.work[wv] = work;
+        s.any[wv] = wave_any;
+    }
+    __syncthreads();
+    if (!(s.any[0] | s.any[1] | s.any[2] | s.any[3])) {
+        if (hdr && threadIdx.x == 0) hdr->merge_blocks = 0;
+        return 0;
+    }
+    work = ((s.work[0] + s.work[1]) + (s.work[2] + s.work[3])) * (float)a.d.n_kv / (float)(2 * gridDim.x);
+    int chunk = (int)fminf(work, 1.0e9f) / 128 * 128 + 128;
     for (;;) {
-        long long items = 0, units = 0, merge = 0;
+        int v[3] = {0, 0, 0}, inc[3], before[3], total[3];  // items, partial units, merge blocks
         for (int r = r0; r < r1; ++r) {
-            const Request q = request(a, r);
+            const Request q = req(r);
             if (!q.m) continue;
-            const Cut c = cut_of<THIN>(a, q, (int)chunk);
+            const Cut c = cut_of<THIN>(a, q, chunk);
             const long long n = (long long)c.nt * a.d.n_kv * c.nc;
-            items += n;
+            v[0] += (int)min(n, 1ll << 30);
             if (c.nc > 1) {
-                units += n * (kTileRows<THIN> / 16);
-                merge += (long long)c.rows * a.d.n_kv;
+                v[1] = (int)min(v[1] + n * (tr / 16), 1ll << 22);  // more than ever fit, and no sum of them wraps
+                v[2] += (c.rows * a.d.n_kv + merge_rows<HDP>(c.nc) - 1) / merge_rows<HDP>(c.nc);
             }
         }
-        long long n_items, n_units, n_merge;
-        long long i0 = block_scan(items, &n_items, s_w), u0 = block_scan(units, &n_units, s_w);
-        if (n_units > units_max && chunk < kMaxChunk) {
-            chunk = min(2 * chunk, (long long)kMaxChunk);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            inc[i] = wave_scan(v[i]);
+            if (lane == 63) s.sum[wv][i] = inc[i];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            before[i] = inc[i] - v[i];
+            total[i] = 0;
+            for (int w = 0; w < 4; ++w) {
+                if (w < wv) before[i] += s.sum[w][i];
+                total[i] += s.sum[w][i];
+            }
+        }
+        if (total[1] > kUnits && chunk < kMaxChunk) {
+            chunk = chunk < kMaxChunk / 2 ? 2 * chunk : kMaxChunk;
+            __syncthreads();  // the sums have been read
             continue;
         }
-        long long m0 = 0;
-        AttnHeader *hdr = blockIdx.x == 0 ? AttnWs<THIN>::header(a.ws) : nullptr;  // one block tells the merge launch
-        if (hdr) m0 = block_scan(merge, &n_merge, s_w);
         for (int r = r0; r < r1; ++r) {
-            s_items[r] = (int)i0;
-            s_units[r] = (int)u0;
+            s_items[r] = before[0];
+            s_units[r] = before[1];
             if (hdr) {
-                hdr->merge[r] = (int)m0;
-                hdr->units[r] = (int)u0;
+                hdr->merge[r] = before[2];
+                hdr->units[r] = before[1];
             }
-            const Request q = request(a, r);
+            const Request q = req(r);
             if (!q.m) continue;
-            const Cut c = cut_of<THIN>(a, q, (int)chunk);
-            const long long n = (long long)c.nt * a.d.n_kv * c.nc;
-            i0 += n;
+            const Cut c = cut_of<THIN>(a, q, chunk);
+            const int n = c.nt * a.d.n_kv * c.nc;
+            before[0] += n;
             if (c.nc > 1) {
-                u0 += n * (kTileRows<THIN> / 16);
-                m0 += (long long)c.rows * a.d.n_kv;
+                before[1] += n * (tr / 16);
+                before[2] += (c.rows * a.d.n_kv + merge_rows<HDP>(c.nc) - 1) / merge_rows<HDP>(c.nc);
             }
         }
         if (threadIdx.x == 0) {
-            s_items[a.n_req] = (int)n_items;
+            s_items[a.n_req] = total[0];
             if (hdr) {
-                hdr->chunk = (int)chunk;
-                hdr->merge_rows = (int)n_merge;
+                hdr->chunk = chunk;
+                hdr->merge_blocks = total[2];
             }
         }
         __syncthreads();
-        return (int)chunk;
+        return chunk;
     }
 }
 
@@ -927,14 +961,14 @@ struct ThinShape {
 template <int HDP>
 __global__ __launch_bounds__(256, (ThinShape<HDP>::PER_CU)) void attn_thin_kernel(AttnArgs a) {
     constexpr int DT = RBT_DT_BF16, WAVE = ThinShape<HDP>::WAVE;
-    __shared__ long long s_w[4];
+    __shared__ ScheduleShared s_sched;
     __shared__ float s_m[4][kThinRows], s_l[4][kThinRows];
     __shared__ int s_flag[kThinRows], s_next;
     int32_t *s_tab = reinterpret_cast<int32_t *>(smem + ThinShape<HDP>::TILE), *s_items = s_tab + kTabPages,
             *s_units = s_items + a.n_req + 1;
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
-    const int chunk = __builtin_amdgcn_readfirstlane(
-        schedule<true>(a, AttnWs<true>::max_units(HDP), s_items, s_units, s_w));
+    const int chunk = __builtin_amdgcn_readfirstlane(schedule<true, HDP>(a, s_items, s_units, s_sched));
+    if (chunk == 0) return;
     ItemQueue items(__builtin_amdgcn_readfirstlane(s_items[a.n_req]), AttnWs<true>::header(a.ws));
     const int span = tab_span(a);
     const PaddedTile<HDP> tl;
@@ -1037,13 +1071,13 @@ struct WideShape {
 template <int DT, int HDP>
 __global__ __launch_bounds__(256, (WideShape<DT, HDP>::PER_CU)) void attn_wide_kernel(AttnArgs a) {
     using Sh = WideShape<DT, HDP>;
-    __shared__ long long s_w[4];
+    __shared__ ScheduleShared s_sched;
     __shared__ int s_flag[kWideRows], s_next;
     int32_t *s_tab = reinterpret_cast<int32_t *>(smem + Sh::TILE), *s_items = s_tab + kTabPages,
             *s_units = s_items + a.n_req + 1;
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
-    const int chunk = __builtin_amdgcn_readfirstlane(
-        schedule<false>(a, AttnWs<false>::max_units(HDP), s_items, s_units, s_w));
+    const int chunk = __builtin_amdgcn_readfirstlane(schedule<false, HDP>(a, s_items, s_units, s_sched));
+    if (chunk == 0) return;
     ItemQueue items(__builtin_amdgcn_readfirstlane(s_items[a.n_req]), AttnWs<false>::header(a.ws));
     const int span = tab_span(a);
     const typename Sh::Tile tl;
@@ -1137,50 +1171,93 @@ __global__ __launch_bounds__(256, (WideShape<DT, HDP>::PER_CU)) void attn_wide_k
     }
 }
 
-// The chunks of cut tiles joined, a wave per row: out = sum_i w_i o_i / sum_i w_i l_i with w_i = 2^(m_i - max m).
+// The pieces of cut tiles joined: out = sum_i w_i o_i / sum_i w_i l_i with w_i = 2^(m_i - max m), HDP / 4 lanes to a row.
 template <int HDP, bool THIN>
-__device__ __forceinline__ void merge_row(const AttnArgs &a, const AttnHeader *hdr, int id) {
-    constexpr int tr = kTileRows<THIN>, tru = tr / 16, VL = HDP / 64;  // VL: floats per lane
-    const int lane = threadIdx.x & 63, r = request_of(hdr->merge, a.n_req, id), chunk = hdr->chunk;
+__device__ __forceinline__ void merge_block(const AttnArgs &a, const AttnHeader *hdr, int id, float (*s_state)[4][2],
+                                            f32x4 (*s_o)[64]) {
+    constexpr int tr = kTileRows<THIN>, tru = tr / 16, LPR = HDP / 4, RPW = 64 / LPR;
+    constexpr size_t step = (size_t)tru * unit_floats(HDP);
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, sub = lane % LPR;
+    const int r = __builtin_amdgcn_readfirstlane(request_of(hdr->merge, a.n_req, id)), chunk = hdr->chunk;
     const Request q = request(a, r);
     const Cut cut = cut_of<THIN>(a, q, chunk);
-    const int local = id - hdr->merge[r], kvh = local / cut.rows, row = local - kvh * cut.rows, tile = row / tr;
+    const bool dealt = cut.nc >= kMergeManyPieces;  // the same for the whole block
+    const int all = cut.rows * a.d.n_kv, mine = (id - hdr->merge[r]) * merge_rows<HDP>(cut.nc) +
+                                                (dealt ? 0 : wv * RPW) + lane / LPR;
+    const int at = min(mine, all - 1), kvh = at / cut.rows, row = at - kvh * cut.rows, tile = row / tr;
     const int row0 = tile * tr, n_rows = min(tr, cut.rows - row0), in = row - row0;
     const int pa = place(a, q, kvh, row0).pos, pb = place(a, q, kvh, row0 + n_rows - 1).pos;
     const int lo = a.window > 0 ? max(0, pa - a.window + 1) : 0;
     const int nc = pieces_of(max(pb + 1 - lo, 0), chunk).n;
-    if (nc == 1) return;  // a tile of a cut request that is not cut itself: written by its block
     const float *u = AttnWs<THIN>::partials(a.ws) +
-                     ((size_t)hdr->units[r] + (size_t)(kvh * cut.nt + tile) * cut.nc * tru + (in >> 4)) * unit_floats(HDP);
-    constexpr size_t step = (size_t)tru * unit_floats(HDP);
+                     ((size_t)hdr->units[r] + (size_t)(kvh * cut.nt + tile) * cut.nc * tru + (in >> 4)) * unit_floats(HDP) +
+                     (in & 15);
+    const float *uo = u - (in & 15) + 32 + (in & 15) * HDP + 4 * sub;
+    const int i0 = dealt ? wv : 0, by = dealt ? 4 : 1;
     float M = -INFINITY;
-    for (int i = lane; i < nc; i += kWave) M = fmaxf(M, u[i * step + (in & 15)]);
-    M = wave_max(M);
-    float L = 0.0f, o[VL] = {};
-    for (int i = 0; i < nc; ++i) {
-        const float w = state_weight(u[i * step + (in & 15)], M);
-        L += w * u[i * step + 16 + (in & 15)];
+    for (int i = i0 + by * sub; i < nc; i += by * LPR) M = fmaxf(M, u[i * step]);
+    for (int x = 1; x < LPR; x <<= 1) M = fmaxf(M, __shfl_xor(M, x, 64));
+    float L = 0.0f;
+    f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    constexpr int kU = 4;  // pieces in flight
+    for (int i = i0; i < nc; i += kU * by) {
+        float m[kU], l[kU];
+        f32x4 v[kU];
 #pragma unroll
-        for (int v = 0; v < VL; ++v) o[v] += w * u[i * step + 32 + (in & 15) * HDP + lane + 64 * v];
+        for (int y = 0; y < kU; ++y) {
+            const size_t p = (size_t)min(i + y * by, nc - 1) * step;
+            m[y] = u[p];
+            l[y] = u[p + 16];
+            v[y] = ld_f4(uo + p);
+        }
+#pragma unroll
+        for (int y = 0; y < kU; ++y)
+            if (i + y * by < nc) {
+                const float w = state_weight(m[y], M);
+                L += w * l[y];
+                o += w * v[y];
+            }
     }
+    if (dealt) {
+        __syncthreads();  // the last states have been read
+        if (sub == 0) {
+            s_state[wv][lane / LPR][0] = M;
+            s_state[wv][lane / LPR][1] = L;
+        }
+        s_o[wv][lane] = o;
+        __syncthreads();
+        if (wv != 0) return;
+        float Mx = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) Mx = fmaxf(Mx, s_state[w][lane / LPR][0]);
+        L = 0.0f;
+        o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float x = state_weight(s_state[w][lane / LPR][0], Mx);
+            L += x * s_state[w][lane / LPR][1];
+            o += x * s_o[w][lane];
+        }
+    }
+    // a tile of a cut request that is not cut itself was written by its block
+    if (mine >= all || nc == 1 || 4 * sub >= a.d.hd) return;
     const Place pl = place(a, q, kvh, row);
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-#pragma unroll
-    for (int v = 0; v < VL; ++v)
-        if (lane + 64 * v < a.d.hd)
-            a.out[(size_t)pl.t * a.out_stride + (size_t)pl.h * a.d.hd + lane + 64 * v] = o[v] * inv;
+    *reinterpret_cast<f32x4 *>(a.out + (size_t)pl.t * a.out_stride + (size_t)pl.h * a.d.hd + 4 * sub) = o * inv;
 }
 // wide: whether the wide launch ran before.
 template <int HDP>
 __global__ __launch_bounds__(256) void attn_merge_kernel(AttnArgs a, int wide) {
+    __shared__ float s_state[4][4][2];
+    __shared__ f32x4 s_o[4][64];
     AttnHeader *hw = AttnWs<false>::header(a.ws), *ht = AttnWs<true>::header(a.ws);
     if (blockIdx.x == 0 && threadIdx.x < 8) hw->taken[threadIdx.x][0] = ht->taken[threadIdx.x][0] = 0;
-    const int nw = wide ? hw->merge_rows : 0, nt = a.thin ? ht->merge_rows : 0;
-    for (int id = blockIdx.x * 4 + (threadIdx.x >> 6); id < nw + nt; id += gridDim.x * 4)
+    const int nw = wide ? hw->merge_blocks : 0, nt = a.thin ? ht->merge_blocks : 0;
+    for (int id = blockIdx.x; id < nw + nt; id += gridDim.x)
         if (id < nt)
-            merge_row<HDP, true>(a, ht, id);
+            merge_block<HDP, true>(a, ht, id, s_state, s_o);
         else
-            merge_row<HDP, false>(a, hw, id - nt);
+            merge_block<HDP, false>(a, hw, id - nt, s_state, s_o);
 }
 
 PagedDims dims_of(const rbt_paged_kv &kv) {
