@@ -369,7 +369,7 @@ __global__ __launch_bounds__(256) void attn_any_kernel(AttnArgs a) {
 // repeat the last one's, with weight 0.
 constexpr int kWideRows = 128, kThinRows = 16;
 constexpr int kTabPages = 1024;  // block numbers of a chunk held in LDS
-constexpr int kMinChunk = 128, kMaxChunk = kPagedMaxLen;  // positions, multiples of 128
+constexpr int kMaxChunk = kPagedMaxLen;  // positions, a multiple of 128
 static_assert(kMaxChunk % 128 == 0, "whole tiles");
 
 // Workspace: for the wide and the thin launch each a header (chunk length, blocks of merging) and the prefix sums of
@@ -390,34 +390,53 @@ struct AttnWs {
     static constexpr int max_units(int hdp) { return (int)((kBytes - sizeof(AttnHeader)) / 4 / unit_floats(hdp)); }
 };
 
-// How a request's rows are cut: tiles of tr rows, each one's positions in nc chunks. rows 0: not this launch's.
-struct Cut {
-    int rows, nt, nc;
-};
+// How a request's rows are cut: nt tiles of tr rows, and each tile's positions into pieces of at most `chunk`. Tile t
+// spans up to S(t) = min(p0 + ceil((t + 1) tr / G), limit) positions, which grow with t, so that tiles from T(c) =
+// floor((c chunk - p0) G / tr) on have more than c pieces. The first c0 pieces are every tile's (T = 0), nc is the
+// last tile's number, and the tiles before t have pieces_before(t) = sum over c of max(0, t - T(c)) in all.
+// rows 0: not this launch's.
 template <bool THIN>
 constexpr int kTileRows = THIN ? kThinRows : kWideRows;
+struct Cut {
+    int rows, nt, nc, c0, p0, limit, chunk, G;
+};
 template <bool THIN>
 __device__ __forceinline__ Cut cut_of(const AttnArgs &a, const Request &q, int chunk) {
     Cut c;
     constexpr int tr = kTileRows<THIN>;
-    const int G = a.n_heads / a.d.n_kv;
-    c.rows = q.m * G;
+    c.G = a.n_heads / a.d.n_kv;
+    c.rows = q.m * c.G;
     if (THIN != (a.thin && c.rows <= kThinRows)) c.rows = 0;
     c.nt = (c.rows + tr - 1) / tr;
-    // a tile's positions: all up to its last row's, or a window's and what its tokens span
-    const int span = a.window > 0 ? min(q.n, min(a.window, q.n) + (tr - 1) / G + 1) : q.n;
-    c.nc = max(1, (int)(((long long)span + chunk - 1) / chunk));
+    c.p0 = q.p0;
+    // all positions up to a tile's last row, or a window's and what its tokens span
+    c.limit = a.window > 0 ? min(q.n, min(a.window, q.n) + (tr - 1) / c.G + 1) : q.n;
+    c.chunk = chunk;
+    c.nc = max(1, (int)(((long long)c.limit + chunk - 1) / chunk));
+    c.c0 = q.p0 > 0 ? min(c.nc, q.p0 / chunk + 1) : 1;
     return c;
 }
-
-// The n pieces of len positions that a tile of span positions is cut into: equal up to whole tiles, none empty (len <=
-// chunk, both multiples of 128).
+template <bool THIN>
+__device__ __forceinline__ int first_with(const Cut &c, int piece) {  // T(piece), for c0 <= piece < nc
+    return (int)(((long long)piece * c.chunk - c.p0) * c.G / kTileRows<THIN>);
+}
+template <bool THIN>
+__device__ __forceinline__ long long pieces_before(const Cut &c, int t) {
+    long long n = (long long)c.c0 * t;
+    for (int i = c.c0; i < c.nc; ++i) n += max(0, t - first_with<THIN>(c, i));
+    return n;
+}
+// Tile t's pieces: n of len positions, equal up to whole tiles of 128 (len <= chunk); the last may be shorter or, where
+// the tile's positions are fewer than S(t), empty.
 struct Pieces {
     int n, len;
 };
-__device__ __forceinline__ Pieces pieces_of(int span, int chunk) {
-    const int n = max(1, (int)(((long long)span + chunk - 1) / chunk));
-    return {n, (int)(((long long)span + n - 1) / n + 127) / 128 * 128};
+template <bool THIN>
+__device__ __forceinline__ Pieces pieces_of(const Cut &c, int t) {
+    const long long rows = min((long long)(t + 1) * kTileRows<THIN>, (long long)c.rows);
+    const int span = max(0, min(c.p0 + (int)((rows + c.G - 1) / c.G), c.limit));
+    const int n = max(1, (int)(((long long)span + c.chunk - 1) / c.chunk));
+    return {n, (int)((((long long)span + n - 1) / n + 127) / 128 * 128)};
 }
 
 // Rows that a block of the merge launch joins: a few per wave, or where many pieces have to be read, as many as one
@@ -483,7 +502,7 @@ __device__ int schedule(const AttnArgs &a, int32_t *s_items, int32_t *s_units, S
             const Request q = req(r);
             if (!q.m) continue;
             const Cut c = cut_of<THIN>(a, q, chunk);
-            const long long n = (long long)c.nt * a.d.n_kv * c.nc;
+            const long long n = pieces_before<THIN>(c, c.nt) * a.d.n_kv;
             v[0] += (int)min(n, 1ll << 30);
             if (c.nc > 1) {
                 v[1] = (int)min(v[1] + n * (tr / 16), 1ll << 22);  // more than ever fit, and no sum of them wraps
@@ -520,7 +539,7 @@ __device__ int schedule(const AttnArgs &a, int32_t *s_items, int32_t *s_units, S
             const Request q = req(r);
             if (!q.m) continue;
             const Cut c = cut_of<THIN>(a, q, chunk);
-            const int n = c.nt * a.d.n_kv * c.nc;
+            const int n = (int)pieces_before<THIN>(c, c.nt) * a.d.n_kv;
             before[0] += n;
             if (c.nc > 1) {
                 before[1] += n * (tr / 16);
@@ -825,7 +844,7 @@ struct Item {
     Request q;
     Cut cut;
     int r, kvh, row0, n_rows, pa, pb, k0, k1;  // rows row0 .. row0 + n_rows - 1 at positions pa .. pb; piece [k0, k1)
-    bool live, split;                          // whether the tile has this piece, and more than one
+    bool split;                                // whether the tile has more than this piece
     float *unit;                               // the piece's partials
 };
 template <bool THIN, int HDP>
@@ -838,50 +857,71 @@ __device__ __forceinline__ Item item_of(const AttnArgs &a, int it, int chunk, co
     x.q = request(a, x.r);
     x.cut = cut_of<THIN>(a, x.q, chunk);
     int local = it - __builtin_amdgcn_readfirstlane(s_items[x.r]);
-    // with a multiple of eight heads each eighth of the items has its own; the longest tiles first, their pieces and
-    // heads together
-    const int hx = a.d.n_kv % 8 == 0 ? a.d.n_kv / 8 : a.d.n_kv, per_group = x.cut.nt * x.cut.nc * hx;
-    const int group = local / per_group;
-    local -= group * per_group;
-    const int tile = x.cut.nt - 1 - local / (x.cut.nc * hx);
-    local %= x.cut.nc * hx;
-    const int c = local / hx;
+    // With a multiple of eight heads each eighth of the items has its own heads. The last pieces of the longest tiles
+    // first, the first piece of the shortest last: a queue that ends with its smallest items leaves no block waiting.
+    const int hx = a.d.n_kv % 8 == 0 ? a.d.n_kv / 8 : a.d.n_kv;
+    const int pieces = (int)pieces_before<THIN>(x.cut, x.cut.nt), group = local / (pieces * hx);
+    local -= group * pieces * hx;
     x.kvh = group * hx + local % hx;
+    local /= hx;
+    int c = x.cut.nc - 1;
+    for (; c >= x.cut.c0; --c) {
+        const int n = x.cut.nt - first_with<THIN>(x.cut, c);
+        if (local < n) break;
+        local -= n;
+    }
+    if (c < x.cut.c0) {
+        c -= local / x.cut.nt;
+        local %= x.cut.nt;
+    }
+    const int tile = x.cut.nt - 1 - local;
     x.row0 = tile * tr;
     x.n_rows = min(tr, x.cut.rows - x.row0);
     x.pa = place(a, x.q, x.kvh, x.row0).pos;
     x.pb = place(a, x.q, x.kvh, x.row0 + x.n_rows - 1).pos;
-    const int lo = a.window > 0 ? max(0, x.pa - a.window + 1) : 0;
-    const Pieces pc = pieces_of(max(x.pb + 1 - lo, 0), chunk);
-    x.live = c < pc.n;
-    x.k0 = x.live ? lo + c * pc.len : 0;
-    x.k1 = x.live ? min(x.pb + 1, x.k0 + min(pc.len, x.pb + 1 - x.k0)) : 0;
+    const int lo = a.window > 0 ? max(0, x.pa - a.window + 1) : 0, end = max(x.pb + 1, lo);
+    const Pieces pc = pieces_of<THIN>(x.cut, tile);
+    x.k0 = (int)min((long long)lo + (long long)c * pc.len, (long long)end);
+    x.k1 = x.k0 + min(pc.len, end - x.k0);
     x.split = pc.n > 1;
     x.unit = AttnWs<THIN>::partials(a.ws) +
              ((size_t)__builtin_amdgcn_readfirstlane(s_units[x.r]) +
-              ((size_t)(x.kvh * x.cut.nt + tile) * x.cut.nc + c) * (tr / 16)) * unit_floats(HDP);
+              ((size_t)x.kvh * pieces + (size_t)pieces_before<THIN>(x.cut, tile) + c) * (tr / 16)) * unit_floats(HDP);
     return x;
 }
 // An eighth of the items to each XCD (blocks b % 8), so that a head's row tiles read its keys and values through one
-// L2. A block starts with the item of its own number and then takes the next one left of its eighth: taken() is asked
-// for early, its answer used by next() at the item's end.
+// L2. A block starts with the item of its own number and then takes the next one left of its eighth, then of the other
+// eighths: ask() early, its answer used by next() at the item's end.
 struct ItemQueue {
-    int it, end, base;
-    int32_t *taken;
-    __device__ __forceinline__ ItemQueue(int n_items, AttnHeader *hdr) {
-        const int xcd = blockIdx.x & 7, i0 = (int)((long long)n_items * xcd / 8);
-        end = (int)((long long)n_items * (xcd + 1) / 8);
-        it = i0 + (int)(blockIdx.x >> 3);
-        base = i0 + (int)(gridDim.x >> 3);
-        taken = &hdr->taken[xcd][0];
+    int it, n, xcd;  // it < 0: nothing is left
+    AttnHeader *hdr;
+    __device__ __forceinline__ int start(int x) const { return (int)((long long)n * x / 8); }
+    __device__ __forceinline__ ItemQueue(int n_items, AttnHeader *header) : n(n_items), xcd(blockIdx.x & 7), hdr(header) {
+        it = start(xcd) + (int)(blockIdx.x >> 3);
+        if (it >= start(xcd + 1)) it = -1;
     }
-    __device__ __forceinline__ int ask() const { return threadIdx.x == 0 ? atomicAdd(taken, 1) : 0; }
-    // for all threads, with a barrier after and before every other use of the shared word
+    __device__ __forceinline__ int ask() const { return threadIdx.x == 0 ? atomicAdd(&hdr->taken[xcd][0], 1) : 0; }
+    // for all threads
     __device__ __forceinline__ void next(int ticket, int *s_next) {
-        if (threadIdx.x == 0) *s_next = ticket;
-        __syncthreads();
-        it = base + __builtin_amdgcn_readfirstlane(*s_next);
-        __syncthreads();
+        const int per = (int)(gridDim.x >> 3);
+        for (;;) {
+            if (threadIdx.x < kWave) {  // the answer, or the first other eighth with any left (its counters only grow)
+                const int x = threadIdx.x & 7;
+                int got = __builtin_amdgcn_readfirstlane(ticket) + start(xcd) + per;
+                if (got >= start(xcd + 1)) {
+                    const int t = __hip_atomic_load(&hdr->taken[x][0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    const uint32_t left = (uint32_t)__ballot(start(x) + per + t < start(x + 1)) & 0xFFu;
+                    got = left ? -2 - (__ffs((int)left) - 1) : -1;
+                }
+                if (threadIdx.x == 0) *s_next = got;
+            }
+            __syncthreads();
+            it = __builtin_amdgcn_readfirstlane(*s_next);
+            __syncthreads();
+            if (it >= -1) return;
+            xcd = -2 - it;
+            ticket = ask();
+        }
     }
 };
 
@@ -972,13 +1012,9 @@ __global__ __launch_bounds__(256, (ThinShape<HDP>::PER_CU)) void attn_thin_kerne
     ItemQueue items(__builtin_amdgcn_readfirstlane(s_items[a.n_req]), AttnWs<true>::header(a.ws));
     const int span = tab_span(a);
     const PaddedTile<HDP> tl;
-    while (items.it < items.end) {
+    while (items.it >= 0) {
         const Item x = item_of<true, HDP>(a, items.it, chunk, s_items, s_units);
         const int ticket = items.ask();
-        if (!x.live) {
-            items.next(ticket, &s_next);
-            continue;
-        }
         WaveState<HDP, 1> w;
         wave_init<HDP, 1>(w, a, x.q, x.cut.rows, x.kvh, x.row0);
         const int k_off = wv * WAVE, v_off = k_off + 32 * PaddedTile<HDP>::ROW;
@@ -1081,13 +1117,9 @@ __global__ __launch_bounds__(256, (WideShape<DT, HDP>::PER_CU)) void attn_wide_k
     ItemQueue items(__builtin_amdgcn_readfirstlane(s_items[a.n_req]), AttnWs<false>::header(a.ws));
     const int span = tab_span(a);
     const typename Sh::Tile tl;
-    while (items.it < items.end) {
+    while (items.it >= 0) {
         const Item x = item_of<false, HDP>(a, items.it, chunk, s_items, s_units);
         const int ticket = items.ask();
-        if (!x.live) {
-            items.next(ticket, &s_next);
-            continue;
-        }
         const int wr0 = x.row0 + 32 * wv;
         const bool active = 32 * wv < x.n_rows;
         const int wa = place(a, x.q, x.kvh, min(wr0, x.cut.rows - 1)).pos,
@@ -1185,12 +1217,11 @@ __device__ __forceinline__ void merge_block(const AttnArgs &a, const AttnHeader 
     const int all = cut.rows * a.d.n_kv, mine = (id - hdr->merge[r]) * merge_rows<HDP>(cut.nc) +
                                                 (dealt ? 0 : wv * RPW) + lane / LPR;
     const int at = min(mine, all - 1), kvh = at / cut.rows, row = at - kvh * cut.rows, tile = row / tr;
-    const int row0 = tile * tr, n_rows = min(tr, cut.rows - row0), in = row - row0;
-    const int pa = place(a, q, kvh, row0).pos, pb = place(a, q, kvh, row0 + n_rows - 1).pos;
-    const int lo = a.window > 0 ? max(0, pa - a.window + 1) : 0;
-    const int nc = pieces_of(max(pb + 1 - lo, 0), chunk).n;
+    const int in = row - tile * tr;
+    const int nc = pieces_of<THIN>(cut, tile).n;
     const float *u = AttnWs<THIN>::partials(a.ws) +
-                     ((size_t)hdr->units[r] + (size_t)(kvh * cut.nt + tile) * cut.nc * tru + (in >> 4)) * unit_floats(HDP) +
+                     ((size_t)hdr->units[r] + ((size_t)kvh * (size_t)pieces_before<THIN>(cut, cut.nt) +
+                                               (size_t)pieces_before<THIN>(cut, tile)) * tru + (in >> 4)) * unit_floats(HDP) +
                      (in & 15);
     const float *uo = u - (in & 15) + 32 + (in & 15) * HDP + 4 * sub;
     const int i0 = dealt ? wv : 0, by = dealt ? 4 : 1;
