@@ -238,7 +238,7 @@ struct AttnArgs {
     PagedDims d;
     int n_req, max_blocks, T, n_heads, window;
     int thin;      // whether requests of up to 16 rows have a launch of their own
-    float scale2;  // scale * log2(e): the softmax runs in powers of two
+    float scale2;  // scale * log2(e), into the query rows: the softmax runs in powers of two
     const int32_t *tables, *kv_len, *q_start;
     const void *kc, *vc;
     const float *q;
@@ -635,35 +635,35 @@ struct WaveState {
 // 32 positions, staged from byte k_off (keys) and v_off (values) of LDS on, parts `part` bytes apart; seen(n): bit 4 t + i, whether query n of this lane sees key 16 t + 4 g + i of them
 // (asked where !full).
 template <int HDP, int NQ, int NP, int part, typename Tile, typename Seen>
-__device__ __forceinline__ void attn_step(WaveState<HDP, NQ> &w, const Tile &tile, int k_off, int v_off, float scale2,
-                                          bool full, Seen seen) {
+__device__ __forceinline__ void attn_step(WaveState<HDP, NQ> &w, const Tile &tile, int k_off, int v_off, bool full,
+                                          Seen seen) {
+    // consecutive products go to different sums: a sum's next product waits for its last
     f32x4 s[NQ][2];
 #pragma unroll
     for (int n = 0; n < NQ; ++n) s[n][0] = s[n][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int st = 0; st < HDP / 32; ++st) {
-        __builtin_amdgcn_sched_barrier(0);
+    for (int st = 0; st < HDP / 32; ++st)
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int kp = 0; kp < NP; ++kp) {
+            u32x4 k[2];
 #pragma unroll
-            for (int kp = 0; kp < NP; ++kp) {
-                const u32x4 k = *reinterpret_cast<const u32x4 *>(smem + (k_off + kp * part) + tile.k_at(t, st));
+            for (int t = 0; t < 2; ++t)
+                k[t] = *reinterpret_cast<const u32x4 *>(smem + (k_off + kp * part) + tile.k_at(t, st));
 #pragma unroll
-                for (int qp = 0; qp + kp < 3; ++qp)
+            for (int qp = 0; qp + kp < 3; ++qp)
 #pragma unroll
-                    for (int n = 0; n < NQ; ++n) s[n][t] = mfma(k, w.q[n][st][qp], s[n][t]);
-            }
-    }
-    __builtin_amdgcn_sched_barrier(0);
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n) s[n][t] = mfma(k[t], w.q[n][st][qp], s[n][t]);
+        }
     if (!full) {
-        const float none = scale2 < 0.0f ? INFINITY : -INFINITY;  // weight 0
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
             const uint32_t bits = seen(n);
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[n][t][i] = bits >> (4 * t + i) & 1 ? s[n][t][i] : none;
+                for (int i = 0; i < 4; ++i) s[n][t][i] = bits >> (4 * t + i) & 1 ? s[n][t][i] : -INFINITY;
         }
     }
     // The reference moves only when a score is 2^8 above it (weights stay below 2^8 then): most steps neither
@@ -676,7 +676,7 @@ __device__ __forceinline__ void attn_step(WaveState<HDP, NQ> &w, const Tile &til
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) top[n] = fmaxf(top[n], s[n][t][i] * scale2);
+            for (int i = 0; i < 4; ++i) top[n] = fmaxf(top[n], s[n][t][i]);
         move |= top[n] > w.m[n] + 8.0f;
     }
     if (__any(move)) {
@@ -699,30 +699,32 @@ __device__ __forceinline__ void attn_step(WaveState<HDP, NQ> &w, const Tile &til
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                e[4 * t + i] = __builtin_amdgcn_exp2f(fmaf(s[n][t][i], scale2, -ref));
+                e[4 * t + i] = __builtin_amdgcn_exp2f(s[n][t][i] - ref);
                 w.l[n] += e[4 * t + i];
             }
         split3(e, p[n]);
     }
 #pragma unroll
-    for (int d = 0; d < HDP / 16; ++d) {
-        if (d % 2 == 0) __builtin_amdgcn_sched_barrier(0);
+    for (int d = 0; d < HDP / 16; d += 2)
 #pragma unroll
         for (int vp = 0; vp < NP; ++vp) {
-            u32x4 v;
+            u32x4 v[2];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const u32x2 h = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (__attribute__((address_space(3))) s16x4 *)(smem + (v_off + vp * part) + tile.v_at(t, d))));
-                v[2 * t] = h[0];
-                v[2 * t + 1] = h[1];
-            }
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const u32x2 h = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (__attribute__((address_space(3))) s16x4 *)(smem + (v_off + vp * part) + tile.v_at(t, d + e))));
+                    v[e][2 * t] = h[0];
+                    v[e][2 * t + 1] = h[1];
+                }
 #pragma unroll
             for (int pp = 0; pp + vp < 3; ++pp)
 #pragma unroll
-                for (int n = 0; n < NQ; ++n) w.o[n][d] = mfma(v, p[n][pp], w.o[n][d]);
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n) w.o[n][d + e] = mfma(v[e], p[n][pp], w.o[n][d + e]);
         }
-    }
 }
 
 // The rows of a wave: rows row0 .. row0 + 16 NQ - 1 of the request (clamped to its last), q in three parts.
@@ -745,8 +747,8 @@ __device__ __forceinline__ void wave_init(WaveState<HDP, NQ> &w, const AttnArgs 
                         x1 = in ? ld_f4(src + 32 * st + 4) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                x[i] = x0[i];
-                x[4 + i] = x1[i];
+                x[i] = x0[i] * a.scale2;
+                x[4 + i] = x1[i] * a.scale2;
             }
             split3(x, w.q[n][st]);
         }
@@ -1030,7 +1032,7 @@ __global__ __launch_bounds__(256, (ThinShape<HDP>::PER_CU)) void attn_thin_kerne
                 __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
                 if (j + 128 < w1) st.load(a, s_tab, page0, x.kvh, j + 128, w1 - 1, lane);
                 const bool full = !bad && j + 32 <= min(w1, x.pa + 1) && (a.window <= 0 || j > x.pb - a.window);
-                attn_step<HDP, 1, 1, 0>(w, tl, k_off, v_off, a.scale2, full,
+                attn_step<HDP, 1, 1, 0>(w, tl, k_off, v_off, full,
                                         [&](int n) { return seen_bits(a, j, w1, w.pos[n], s_tab, page0, bad); });
             }
         }
@@ -1137,7 +1139,7 @@ __global__ __launch_bounds__(256, (WideShape<DT, HDP>::PER_CU)) void attn_wide_k
                     const bool full = !bad && j + 32 <= min(w1, wa + 1) && (a.window <= 0 || j > wb - a.window);
                     const int k_off = buf + u * Sh::Tile::ROW;
                     attn_step<HDP, 2, Sh::NP, Sh::PART>(
-                        w, tl, k_off, k_off + Sh::NP * Sh::PART, a.scale2, full,
+                        w, tl, k_off, k_off + Sh::NP * Sh::PART, full,
                         [&](int n) { return seen_bits(a, j, w1, w.pos[n], s_tab, page0, bad); });
                 }
             };
