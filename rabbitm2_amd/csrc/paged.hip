@@ -637,25 +637,46 @@ struct WaveState {
 template <int HDP, int NQ, int NP, int part, typename Tile, typename Seen>
 __device__ __forceinline__ void attn_step(WaveState<HDP, NQ> &w, const Tile &tile, int k_off, int v_off, bool full,
                                           Seen seen) {
-    // consecutive products go to different sums: a sum's next product waits for its last
+    // Consecutive products go to different sums: a sum's next product waits for its last. The operands of the next
+    // products are read from LDS before those of the last ones are used.
+    constexpr int KI = HDP / 32 * NP, VI = HDP / 32 * NP;  // (k-step, part) and (pair of 16 dims, part)
+    auto read_k = [&](int i, u32x4 (&k)[2]) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+            k[t] = *reinterpret_cast<const u32x4 *>(smem + (k_off + i % NP * part) + tile.k_at(t, i / NP));
+    };
+    auto read_v = [&](int i, u32x4 (&v)[2]) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const u32x2 h = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (__attribute__((address_space(3))) s16x4 *)(smem + (v_off + i % NP * part) +
+                                                                tile.v_at(t, i / NP * 2 + e))));
+                v[e][2 * t] = h[0];
+                v[e][2 * t + 1] = h[1];
+            }
+    };
     f32x4 s[NQ][2];
 #pragma unroll
     for (int n = 0; n < NQ; ++n) s[n][0] = s[n][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    u32x4 k[2][2], v[2][2];
+    read_k(0, k[0]);
 #pragma unroll
-    for (int st = 0; st < HDP / 32; ++st)
+    for (int i = 0; i < KI; ++i) {
+        if (i + 1 < KI)
+            read_k(i + 1, k[(i + 1) & 1]);
+        else
+            read_v(0, v[0]);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int kp = 0; kp < NP; ++kp) {
-            u32x4 k[2];
+        for (int qp = 0; qp + i % NP < 3; ++qp)
 #pragma unroll
             for (int t = 0; t < 2; ++t)
-                k[t] = *reinterpret_cast<const u32x4 *>(smem + (k_off + kp * part) + tile.k_at(t, st));
 #pragma unroll
-            for (int qp = 0; qp + kp < 3; ++qp)
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int n = 0; n < NQ; ++n) s[n][t] = mfma(k[t], w.q[n][st][qp], s[n][t]);
-        }
+                for (int n = 0; n < NQ; ++n) s[n][t] = mfma(k[i & 1][t], w.q[n][i / NP][qp], s[n][t]);
+        __builtin_amdgcn_sched_barrier(0);
+    }
     if (!full) {
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
@@ -705,26 +726,20 @@ __device__ __forceinline__ void attn_step(WaveState<HDP, NQ> &w, const Tile &til
         split3(e, p[n]);
     }
 #pragma unroll
-    for (int d = 0; d < HDP / 16; d += 2)
+    for (int i = 0; i < VI; ++i) {
+        if (i + 1 < VI) read_v(i + 1, v[(i + 1) & 1]);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int vp = 0; vp < NP; ++vp) {
-            u32x4 v[2];
+        for (int pp = 0; pp + i % NP < 3; ++pp)
 #pragma unroll
             for (int e = 0; e < 2; ++e)
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const u32x2 h = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (__attribute__((address_space(3))) s16x4 *)(smem + (v_off + vp * part) + tile.v_at(t, d + e))));
-                    v[e][2 * t] = h[0];
-                    v[e][2 * t + 1] = h[1];
+                for (int n = 0; n < NQ; ++n) {
+                    f32x4 &o = w.o[n][i / NP * 2 + e];
+                    o = mfma(v[i & 1][e], p[n][pp], o);
                 }
-#pragma unroll
-            for (int pp = 0; pp + vp < 3; ++pp)
-#pragma unroll
-                for (int e = 0; e < 2; ++e)
-#pragma unroll
-                    for (int n = 0; n < NQ; ++n) w.o[n][d + e] = mfma(v[e], p[n][pp], w.o[n][d + e]);
-        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
 }
 
 // The rows of a wave: rows row0 .. row0 + 16 NQ - 1 of the request (clamped to its last), q in three parts.
@@ -759,7 +774,12 @@ __device__ __forceinline__ void wave_init(WaveState<HDP, NQ> &w, const AttnArgs 
 
 // Staging of KEYS positions from j on (those past last repeat it) by THREADS threads: 16-byte chunks of 8 elements
 // through registers, so that a tile's loads run during the arithmetic of the one before.
-template <int DT, int HDP, int KEYS, int THREADS>
+// ONCE: keys and values that one block alone reads stream past the caches.
+template <bool ONCE>
+__device__ __forceinline__ u32x4 ld_kv(const uint8_t *p) {
+    return ONCE ? ld_stream_u4(p) : *reinterpret_cast<const u32x4 *>(p);
+}
+template <int DT, int HDP, int KEYS, int THREADS, bool ONCE>
 struct Stage {
     static constexpr int CH = HDP / 8, ROWS = THREADS / CH, N = KEYS / ROWS;
     static constexpr int LD = DT == RBT_DT_BF16 ? 1 : 2;
@@ -780,8 +800,8 @@ struct Stage {
             for (int x = 0; x < LD; ++x) {
                 k[i][x] = v[i][x] = u32x4{0, 0, 0, 0};
                 if (in) {
-                    k[i][x] = *reinterpret_cast<const u32x4 *>(static_cast<const uint8_t *>(a.kc) + at + 16 * x);
-                    v[i][x] = *reinterpret_cast<const u32x4 *>(static_cast<const uint8_t *>(a.vc) + at + 16 * x);
+                    k[i][x] = ld_kv<ONCE>(static_cast<const uint8_t *>(a.kc) + at + 16 * x);
+                    v[i][x] = ld_kv<ONCE>(static_cast<const uint8_t *>(a.vc) + at + 16 * x);
                 }
             }
         }
@@ -1023,7 +1043,7 @@ __global__ __launch_bounds__(256, (ThinShape<HDP>::PER_CU)) void attn_thin_kerne
         for (int w0 = x.k0; w0 < x.k1; w0 += span) {
             const int w1 = min(x.k1, w0 + min(span, x.k1 - w0)), page0 = (int)page_of((uint32_t)w0, a.d.div);
             const bool bad = fill_tab(a, x.r, w0, w1, s_tab);
-            Stage<DT, HDP, 32, 64> st;
+            Stage<DT, HDP, 32, 64, true> st;
             int j = w0 + 32 * wv;
             if (j < w1) st.load(a, s_tab, page0, x.kvh, j, w1 - 1, lane);
             for (; j < w1; j += 128) {
@@ -1155,7 +1175,7 @@ __global__ __launch_bounds__(256, (WideShape<DT, HDP>::PER_CU)) void attn_wide_k
                     buf ^= Sh::BUF;
                 }
             } else {
-                Stage<DT, HDP, Sh::KEYS, 256> st;
+                Stage<DT, HDP, Sh::KEYS, 256, false> st;
                 st.load(a, s_tab, page0, x.kvh, w0, w1 - 1, tid);
                 for (int jt = w0; jt < w1; jt += Sh::KEYS) {
                     __syncthreads();
