@@ -237,6 +237,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
 struct AttnArgs {
     PagedDims d;
     int n_req, max_blocks, T, n_heads, window;
+    PageDiv group; // query heads to a key/value head
     int thin;      // whether requests of up to 16 rows have a launch of their own
     float scale2;  // scale * log2(e), into the query rows: the softmax runs in powers of two
     const int32_t *tables, *kv_len, *q_start;
@@ -271,7 +272,7 @@ template <int DT>
 __device__ void row_any(const AttnArgs &a, RowShared &s, int r, int t, int h, int j0, int j1, float *m_out, float *l_out,
                         float *o_out) {
     constexpr uint64_t kNone = ~0ull;
-    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, hd = a.d.hd, kvh = h / (a.n_heads / a.d.n_kv);
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, hd = a.d.hd, kvh = h / (int)a.group.d;
     __syncthreads();  // the shared values of a previous call have been read
     if (tid < hd) s.q[tid] = a.q[(size_t)t * a.q_stride + (size_t)h * hd + tid];
     __syncthreads();
@@ -368,7 +369,7 @@ __global__ __launch_bounds__(256) void attn_any_kernel(AttnArgs a) {
 // result is not finite are computed again by row_any, which reads seen positions only. Rows past the positions
 // repeat the last one's, with weight 0.
 constexpr int kWideRows = 128, kThinRows = 16;
-constexpr int kTabPages = 1024;  // block numbers of a chunk held in LDS
+constexpr int kTabPages = 512;  // pages whose places are held in LDS at a time
 constexpr int kMaxChunk = kPagedMaxLen;  // positions, a multiple of 128
 static_assert(kMaxChunk % 128 == 0, "whole tiles");
 
@@ -404,7 +405,7 @@ template <bool THIN>
 __device__ __forceinline__ Cut cut_of(const AttnArgs &a, const Request &q, int chunk) {
     Cut c;
     constexpr int tr = kTileRows<THIN>;
-    c.G = a.n_heads / a.d.n_kv;
+    c.G = (int)a.group.d;
     c.rows = q.m * c.G;
     if (THIN != (a.thin && c.rows <= kThinRows)) c.rows = 0;
     c.nt = (c.rows + tr - 1) / tr;
@@ -632,11 +633,11 @@ struct WaveState {
     int pos[NQ];  // this lane's query's position
 };
 
-// 32 positions, staged from byte k_off (keys) and v_off (values) of LDS on, parts `part` bytes apart; seen(n): bit 4 t + i, whether query n of this lane sees key 16 t + 4 g + i of them
+// 32 positions, staged from byte k_off (keys) and v_off (values) of LDS on, parts `part` bytes apart; between(i) is called among the products, for i = 0 .. HDP / 16 NP - 1 in turn; seen(n): bit 4 t + i, whether query n of this lane sees key 16 t + 4 g + i of them
 // (asked where !full).
-template <int HDP, int NQ, int NP, int part, typename Tile, typename Seen>
+template <int HDP, int NQ, int NP, int part, typename Tile, typename Between, typename Seen>
 __device__ __forceinline__ void attn_step(WaveState<HDP, NQ> &w, const Tile &tile, int k_off, int v_off, bool full,
-                                          Seen seen) {
+                                          Between between, Seen seen) {
     // Consecutive products go to different sums: a sum's next product waits for its last. The operands of the next
     // products are read from LDS before those of the last ones are used.
     constexpr int KI = HDP / 32 * NP, VI = HDP / 32 * NP;  // (k-step, part) and (pair of 16 dims, part)
@@ -668,6 +669,7 @@ __device__ __forceinline__ void attn_step(WaveState<HDP, NQ> &w, const Tile &til
             read_k(i + 1, k[(i + 1) & 1]);
         else
             read_v(0, v[0]);
+        between(i);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int qp = 0; qp + i % NP < 3; ++qp)
@@ -728,6 +730,7 @@ __device__ __forceinline__ void attn_step(WaveState<HDP, NQ> &w, const Tile &til
 #pragma unroll
     for (int i = 0; i < VI; ++i) {
         if (i + 1 < VI) read_v(i + 1, v[(i + 1) & 1]);
+        between(KI + i);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int pp = 0; pp + i % NP < 3; ++pp)
@@ -746,10 +749,11 @@ __device__ __forceinline__ void attn_step(WaveState<HDP, NQ> &w, const Tile &til
 template <int HDP, int NQ>
 __device__ __forceinline__ void wave_init(WaveState<HDP, NQ> &w, const AttnArgs &a, const Request &q, int rows, int kvh,
                                           int row0) {
-    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, G = a.n_heads / a.d.n_kv;
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, G = (int)a.group.d;
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-        const int row = min(row0 + 16 * n + c, rows - 1), tok = row / G, h = kvh * G + row - tok * G;
+        const int row = min(row0 + 16 * n + c, rows - 1), tok = (int)page_of((uint32_t)row, a.group);
+        const int h = kvh * G + row - tok * G;
         const float *src = a.q + (size_t)(q.t0 + tok) * a.q_stride + (size_t)h * a.d.hd + 8 * g;
         w.pos[n] = q.p0 + tok;
         w.m[n] = -INFINITY;
@@ -772,6 +776,38 @@ __device__ __forceinline__ void wave_init(WaveState<HDP, NQ> &w, const AttnArgs 
     }
 }
 
+// The places (byte offset of the block) of the pages that positions j0 .. j1 - 1 (at most tab_span of them) lie on, into
+// s_tab; 1 for a page outside the cache (whose positions are read from offset 0 and not seen): whether there is any.
+// For all threads of the block.
+constexpr int kTabBytes = 8 * kTabPages;
+__device__ __forceinline__ int tab_span(const AttnArgs &a) {
+    return (int)(min((kTabPages - 1) * (long long)a.d.block_size, (long long)kMaxChunk) / 128 * 128);
+}
+template <int DT>
+__device__ __forceinline__ bool fill_tab(const AttnArgs &a, int r, int j0, int j1, uint64_t *s_tab) {
+    const int page0 = (int)page_of((uint32_t)j0, a.d.div), n = (int)page_of((uint32_t)(j1 - 1), a.d.div) - page0 + 1;
+    bool bad = false;
+    __syncthreads();  // the last table has been read
+    for (int i = threadIdx.x; i < n; i += 256) {
+        const int b = a.tables[(size_t)r * a.max_blocks + page0 + i];
+        const bool ok = b >= 0 && b < a.d.n_blocks;
+        bad |= !ok;
+        s_tab[i] = ok ? (uint64_t)b * a.d.block_stride * (DT == RBT_DT_BF16 ? 2 : 4) : 1;
+    }
+    return __builtin_amdgcn_readfirstlane(__syncthreads_or(bad)) != 0;
+}
+// Where a position's row of a head (head_off: the head's bytes in a block) lies in the cache.
+template <int DT>
+__device__ __forceinline__ uint64_t row_at(const AttnArgs &a, const uint64_t *s_tab, int page0, uint32_t head_off, int pos) {
+    const int page = (int)page_of((uint32_t)pos, a.d.div);
+    const uint32_t in = (uint32_t)(pos - page * a.d.block_size) * (uint32_t)(a.d.hd * (DT == RBT_DT_BF16 ? 2 : 4));
+    return (s_tab[page - page0] & ~(uint64_t)15) + (head_off + in);
+}
+template <int DT>
+__device__ __forceinline__ uint32_t head_offset(const AttnArgs &a, int kvh) {
+    return (uint32_t)kvh * (uint32_t)a.d.block_size * (uint32_t)(a.d.hd * (DT == RBT_DT_BF16 ? 2 : 4));
+}
+
 // Staging of KEYS positions from j on (those past last repeat it) by THREADS threads: 16-byte chunks of 8 elements
 // through registers, so that a tile's loads run during the arithmetic of the one before.
 // ONCE: keys and values that one block alone reads stream past the caches.
@@ -786,16 +822,15 @@ struct Stage {
     static_assert(N * ROWS == KEYS, "whole passes");
     u32x4 k[N][LD], v[N][LD];
 
-    __device__ __forceinline__ void load(const AttnArgs &a, const int32_t *s_tab, int page0, int kvh, int j, int last,
+    __device__ __forceinline__ void load(const AttnArgs &a, const uint64_t *s_tab, int page0, int kvh, int j, int last,
                                          int tid) {
         const int row = tid / CH, chunk = tid % CH;
+        const uint32_t head_off = head_offset<DT>(a, kvh);
         const bool in = 8 * chunk < a.d.hd;
         constexpr size_t esz = DT == RBT_DT_BF16 ? 2 : 4;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int key = min(j + row + i * ROWS, last), page = (int)page_of((uint32_t)key, a.d.div);
-            const int b = max(s_tab[page - page0], 0);
-            const uint64_t at = (paged_row(a.d, b, kvh, key - page * a.d.block_size) + 8 * chunk) * esz;
+            const uint64_t at = row_at<DT>(a, s_tab, page0, head_off, min(j + row + i * ROWS, last)) + 8 * chunk * esz;
 #pragma unroll
             for (int x = 0; x < LD; ++x) {
                 k[i][x] = v[i][x] = u32x4{0, 0, 0, 0};
@@ -830,34 +865,41 @@ struct Stage {
     }
 };
 
-// The same for a bf16 tile of a block's four waves as direct copies into LDS (SwizzledTile), not waited for. A head
-// dim below HDP: the chunks behind it repeat its last (the query's are 0, and the output's are not stored).
+// The same for a bf16 tile of a block's four waves as direct copies into LDS (SwizzledTile), not waited for: aim() finds
+// the places, copy(i) makes the i-th of a wave's COPIES. A copy holds up its wave while the ones before it are taken
+// (32 KiB at 64 bytes a clock), so they are made one by one among the products of the tile before. A head dim below HDP:
+// the chunks behind it repeat its last (the query's are 0, and the output's are not stored).
 template <int HDP, int KEYS>
-__device__ __forceinline__ void copy_tile(const AttnArgs &a, const int32_t *s_tab, int page0, int kvh, int j, int last,
-                                          int buf) {
+struct TileCopy {
     using Tile = SwizzledTile<HDP>;
-    constexpr int ROWS = 64 / Tile::CH, N = KEYS / 4 / ROWS;  // rows per copy, copies per wave (of K, of V)
+    static constexpr int ROWS = 64 / Tile::CH, N = KEYS / 4 / ROWS, COPIES = 2 * N;  // rows per copy
     static_assert(N * 4 * ROWS == KEYS, "whole copies");
-    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)smem + (uint32_t)buf;
+    uint64_t at[N];
+    uint32_t lds;
+    __device__ __forceinline__ void aim(const AttnArgs &a, const uint64_t *s_tab, int page0, int kvh, int j, int last,
+                                        int buf) {
+        const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+        const uint32_t head_off = head_offset<RBT_DT_BF16>(a, kvh);
+        lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)smem + (uint32_t)(buf + wv * N * ROWS * Tile::ROW);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int row0 = (wv * N + i) * ROWS, row = row0 + lane / Tile::CH;
-        const int chunk = min((lane % Tile::CH) ^ Tile::key(row), a.d.hd / 8 - 1);
-        const int pos = min(j + row, last), page = (int)page_of((uint32_t)pos, a.d.div);
-        const int b = max(s_tab[page - page0], 0);
-        const uint64_t at = (paged_row(a.d, b, kvh, pos - page * a.d.block_size) + 8 * chunk) * 2;
-        lds_dma16(static_cast<const uint8_t *>(a.kc) + at, lds + (uint32_t)(row0 * Tile::ROW));
-        lds_dma16(static_cast<const uint8_t *>(a.vc) + at, lds + (uint32_t)((KEYS + row0) * Tile::ROW));
+        for (int i = 0; i < N; ++i) {
+            const int row = (wv * N + i) * ROWS + lane / Tile::CH;
+            const int chunk = min((lane % Tile::CH) ^ Tile::key(row), a.d.hd / 8 - 1);
+            at[i] = row_at<RBT_DT_BF16>(a, s_tab, page0, head_off, min(j + row, last)) + 16 * chunk;
+        }
     }
-}
+    __device__ __forceinline__ void copy(const AttnArgs &a, int i) const {
+        const uint8_t *src = static_cast<const uint8_t *>(i & 1 ? a.vc : a.kc);
+        lds_dma16(src + at[i / 2], lds + (uint32_t)(((i & 1) * KEYS + i / 2 * ROWS) * Tile::ROW));
+    }
+};
 
 // A row's place: its token and head.
 struct Place {
     int t, h, pos;
 };
 __device__ __forceinline__ Place place(const AttnArgs &a, const Request &q, int kvh, int row) {
-    const int G = a.n_heads / a.d.n_kv, tok = row / G;
+    const int G = (int)a.group.d, tok = (int)page_of((uint32_t)row, a.group);
     return {q.t0 + tok, kvh * G + row - tok * G, q.p0 + tok};
 }
 
@@ -947,27 +989,8 @@ struct ItemQueue {
     }
 };
 
-// Block numbers of the pages that positions j0 .. j1 - 1 (at most tab_span of them) lie on, into s_tab; -1 for one
-// outside the cache: whether there is any. For all threads of the block.
-constexpr int kTabBytes = 4 * kTabPages;
-__device__ __forceinline__ int tab_span(const AttnArgs &a) {
-    return (int)(min((kTabPages - 1) * (long long)a.d.block_size, (long long)kMaxChunk) / 128 * 128);
-}
-__device__ __forceinline__ bool fill_tab(const AttnArgs &a, int r, int j0, int j1, int32_t *s_tab) {
-    const int page0 = (int)page_of((uint32_t)j0, a.d.div), n = (int)page_of((uint32_t)(j1 - 1), a.d.div) - page0 + 1;
-    bool bad = false;
-    __syncthreads();  // the last table has been read
-    for (int i = threadIdx.x; i < n; i += 256) {
-        const int b = a.tables[(size_t)r * a.max_blocks + page0 + i];
-        const bool ok = b >= 0 && b < a.d.n_blocks;
-        bad |= !ok;
-        s_tab[i] = ok ? b : -1;
-    }
-    return __builtin_amdgcn_readfirstlane(__syncthreads_or(bad)) != 0;
-}
-
 // Which of a lane's 16 t + 4 g + i (bit 4 t + i) of 32 positions from j on the query at pos sees.
-__device__ __forceinline__ uint32_t seen_bits(const AttnArgs &a, int j, int k1, int pos, const int32_t *s_tab, int page0,
+__device__ __forceinline__ uint32_t seen_bits(const AttnArgs &a, int j, int k1, int pos, const uint64_t *s_tab, int page0,
                                               bool bad) {
     const int g = (threadIdx.x & 63) >> 4;
     const int first = a.window > 0 ? pos - a.window : -1, last = min(k1 - 1, pos);
@@ -980,7 +1003,7 @@ __device__ __forceinline__ uint32_t seen_bits(const AttnArgs &a, int j, int k1, 
     if (bad)
         for (int e = 0; e < 8; ++e) {
             const int key = min(j + 16 * (e >> 2) + 4 * g + (e & 3), k1 - 1);
-            if (s_tab[(int)page_of((uint32_t)key, a.d.div) - page0] < 0) bits &= ~(1u << e);
+            if (s_tab[(int)page_of((uint32_t)key, a.d.div) - page0] & 1) bits &= ~(1u << e);
         }
     return bits;
 }
@@ -1007,7 +1030,7 @@ __device__ __forceinline__ void again_rows(const AttnArgs &a, const Item &x, con
     }
 }
 
-// LDS: [tile | row_any's][block numbers][item and unit prefix sums]
+// LDS: [tile | row_any's][pages' places][item and unit prefix sums]
 constexpr int kLdsBytes = 159 << 10;  // of 160 KiB: the kernels' fixed shared variables take less than the last
 constexpr int attn_lds(int tile, int n_req) { return tile + kTabBytes + 8 * (n_req + 1); }
 
@@ -1026,8 +1049,8 @@ __global__ __launch_bounds__(256, (ThinShape<HDP>::PER_CU)) void attn_thin_kerne
     __shared__ ScheduleShared s_sched;
     __shared__ float s_m[4][kThinRows], s_l[4][kThinRows];
     __shared__ int s_flag[kThinRows], s_next;
-    int32_t *s_tab = reinterpret_cast<int32_t *>(smem + ThinShape<HDP>::TILE), *s_items = s_tab + kTabPages,
-            *s_units = s_items + a.n_req + 1;
+    uint64_t *s_tab = reinterpret_cast<uint64_t *>(smem + ThinShape<HDP>::TILE);
+    int32_t *s_items = reinterpret_cast<int32_t *>(s_tab + kTabPages), *s_units = s_items + a.n_req + 1;
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
     const int chunk = __builtin_amdgcn_readfirstlane(schedule<true, HDP>(a, s_items, s_units, s_sched));
     if (chunk == 0) return;
@@ -1042,7 +1065,7 @@ __global__ __launch_bounds__(256, (ThinShape<HDP>::PER_CU)) void attn_thin_kerne
         const int k_off = wv * WAVE, v_off = k_off + 32 * PaddedTile<HDP>::ROW;
         for (int w0 = x.k0; w0 < x.k1; w0 += span) {
             const int w1 = min(x.k1, w0 + min(span, x.k1 - w0)), page0 = (int)page_of((uint32_t)w0, a.d.div);
-            const bool bad = fill_tab(a, x.r, w0, w1, s_tab);
+            const bool bad = fill_tab<DT>(a, x.r, w0, w1, s_tab);
             Stage<DT, HDP, 32, 64, true> st;
             int j = w0 + 32 * wv;
             if (j < w1) st.load(a, s_tab, page0, x.kvh, j, w1 - 1, lane);
@@ -1052,7 +1075,7 @@ __global__ __launch_bounds__(256, (ThinShape<HDP>::PER_CU)) void attn_thin_kerne
                 __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
                 if (j + 128 < w1) st.load(a, s_tab, page0, x.kvh, j + 128, w1 - 1, lane);
                 const bool full = !bad && j + 32 <= min(w1, x.pa + 1) && (a.window <= 0 || j > x.pb - a.window);
-                attn_step<HDP, 1, 1, 0>(w, tl, k_off, v_off, full,
+                attn_step<HDP, 1, 1, 0>(w, tl, k_off, v_off, full, [](int) {},
                                         [&](int n) { return seen_bits(a, j, w1, w.pos[n], s_tab, page0, bad); });
             }
         }
@@ -1117,10 +1140,11 @@ __global__ __launch_bounds__(256, (ThinShape<HDP>::PER_CU)) void attn_thin_kerne
 template <int DT, int HDP>
 struct WideShape {
     static constexpr int NP = DT == RBT_DT_BF16 ? 1 : 3;
-    static constexpr int KEYS = DT == RBT_DT_BF16 && HDP <= 128 ? 64 : 32;
+    static constexpr int KEYS = 32;
     // bf16: two buffers that direct copies fill in turn; f32: one of parts, through registers
     static constexpr bool COPY = DT == RBT_DT_BF16;
     using Tile = std::conditional_t<COPY, SwizzledTile<HDP>, PaddedTile<HDP>>;
+    static_assert(COPY || KEYS == 32, "a tile of parts is one step");
     static constexpr int PART = KEYS * Tile::ROW, BUF = 2 * NP * PART;
     static constexpr int TILE = COPY ? 2 * BUF : BUF;
     static constexpr int PER_CU = HDP <= 128 ? 2 : 1;
@@ -1131,8 +1155,8 @@ __global__ __launch_bounds__(256, (WideShape<DT, HDP>::PER_CU)) void attn_wide_k
     using Sh = WideShape<DT, HDP>;
     __shared__ ScheduleShared s_sched;
     __shared__ int s_flag[kWideRows], s_next;
-    int32_t *s_tab = reinterpret_cast<int32_t *>(smem + Sh::TILE), *s_items = s_tab + kTabPages,
-            *s_units = s_items + a.n_req + 1;
+    uint64_t *s_tab = reinterpret_cast<uint64_t *>(smem + Sh::TILE);
+    int32_t *s_items = reinterpret_cast<int32_t *>(s_tab + kTabPages), *s_units = s_items + a.n_req + 1;
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
     const int chunk = __builtin_amdgcn_readfirstlane(schedule<false, HDP>(a, s_items, s_units, s_sched));
     if (chunk == 0) return;
@@ -1150,28 +1174,35 @@ __global__ __launch_bounds__(256, (WideShape<DT, HDP>::PER_CU)) void attn_wide_k
         wave_init<HDP, 2>(w, a, x.q, x.cut.rows, x.kvh, wr0);
         for (int w0 = x.k0; w0 < x.k1; w0 += span) {
             const int w1 = min(x.k1, w0 + min(span, x.k1 - w0)), page0 = (int)page_of((uint32_t)w0, a.d.div);
-            const bool bad = fill_tab(a, x.r, w0, w1, s_tab);
-            // the wave's part of a staged tile from position jt on
-            auto steps = [&](int jt, int buf) {
-                for (int u = 0; u < Sh::KEYS; u += 32) {
-                    const int j = jt + u;
-                    if (!active || j >= w1 || j > wb || (a.window > 0 && j + 31 <= wa - a.window)) continue;
-                    const bool full = !bad && j + 32 <= min(w1, wa + 1) && (a.window <= 0 || j > wb - a.window);
-                    const int k_off = buf + u * Sh::Tile::ROW;
-                    attn_step<HDP, 2, Sh::NP, Sh::PART>(
-                        w, tl, k_off, k_off + Sh::NP * Sh::PART, full,
-                        [&](int n) { return seen_bits(a, j, w1, w.pos[n], s_tab, page0, bad); });
-                }
+            const bool bad = fill_tab<DT>(a, x.r, w0, w1, s_tab);
+            // the wave's part of 32 staged positions from j on: whether it has any
+            auto step = [&](int j, int off, auto between) {
+                if (!active || j >= w1 || j > wb || (a.window > 0 && j + 31 <= wa - a.window)) return false;
+                const bool full = !bad && j + 32 <= min(w1, wa + 1) && (a.window <= 0 || j > wb - a.window);
+                attn_step<HDP, 2, Sh::NP, Sh::PART>(
+                    w, tl, off, off + Sh::NP * Sh::PART, full, between,
+                    [&](int n) { return seen_bits(a, j, w1, w.pos[n], s_tab, page0, bad); });
+                return true;
             };
             if constexpr (Sh::COPY) {
-                copy_tile<HDP, Sh::KEYS>(a, s_tab, page0, x.kvh, w0, w1 - 1, 0);
+                TileCopy<HDP, Sh::KEYS> cp;
+                static_assert(cp.COPIES <= HDP / 16, "a step has room for a tile's copies");
+                auto copies = [&]() {
+#pragma unroll
+                    for (int i = 0; i < cp.COPIES; ++i) cp.copy(a, i);
+                };
+                cp.aim(a, s_tab, page0, x.kvh, w0, w1 - 1, 0);
+                copies();
                 int buf = 0;
                 for (int jt = w0; jt < w1; jt += Sh::KEYS) {
                     wait_dma<0>();
                     __syncthreads();  // this tile has landed for all, and the last one has been read
-                    if (jt + Sh::KEYS < w1)
-                        copy_tile<HDP, Sh::KEYS>(a, s_tab, page0, x.kvh, jt + Sh::KEYS, w1 - 1, buf ^ Sh::BUF);
-                    steps(jt, buf);
+                    const bool more = jt + Sh::KEYS < w1;
+                    if (more) cp.aim(a, s_tab, page0, x.kvh, jt + Sh::KEYS, w1 - 1, buf ^ Sh::BUF);
+                    if (more) copies();
+                    step(jt, buf, [](int) {});
+#pragma unroll
+                    for (int u = 32; u < Sh::KEYS; u += 32) step(jt + u, buf + u * Sh::Tile::ROW, [](int) {});
                     buf ^= Sh::BUF;
                 }
             } else {
@@ -1182,7 +1213,7 @@ __global__ __launch_bounds__(256, (WideShape<DT, HDP>::PER_CU)) void attn_wide_k
                     st.store(0, Sh::NP * Sh::PART, Sh::PART, tid);
                     __syncthreads();
                     if (jt + Sh::KEYS < w1) st.load(a, s_tab, page0, x.kvh, jt + Sh::KEYS, w1 - 1, tid);
-                    steps(jt, 0);
+                    step(jt, 0, [](int) {});
                 }
             }
         }
@@ -1435,6 +1466,7 @@ hipError_t launch_paged_attn(const Launch &L, const Launch &Lm, const rbt_paged_
     a.max_blocks = b.max_blocks;
     a.T = T;
     a.n_heads = n_heads;
+    a.group = page_div(n_heads / kv.n_kv_heads);
     a.window = window;
     a.scale2 = scale * 1.44269504088896340736f;
     a.tables = b.tables;
