@@ -361,9 +361,8 @@ __global__ __launch_bounds__(256) void attn_any_kernel(AttnArgs a) {
 // the B operand of O^T = V^T P^T whose k-slot (g, 4 t + i) is key 16 t + 4 g + i. V^T comes from the row-major
 // tile by the transposing LDS read (ds_read_b64_tr_b16: lane c of group g gets column c of rows 4 g .. 4 g + 3).
 //
-// Precision: bf16 keys and values enter exactly. f32 operands are cut into three bf16 parts of 8 bits each by
-// truncation (exact for all normal values: 24 bits), and the products of parts down to 2^-24 are taken: three for
-// a bf16 cache, six for an f32 one. Sums, the softmax and its state are f32.
+// Precision: bf16 keys and values enter exactly. f32 operands are cut into three bf16 parts of 8 bits each (exact: 24
+// bits), and the products of parts down to 2^-24 are taken: three for a bf16 cache, six for an f32 one. Sums, the softmax and its state are f32.
 //
 // Not finite: a position that a row does not see has weight 0, but 0 times an infinity is NaN, so rows whose
 // result is not finite are computed again by row_any, which reads seen positions only. Rows past the positions
@@ -413,7 +412,7 @@ __device__ __forceinline__ Cut cut_of(const AttnArgs &a, const Request &q, int c
     // all positions up to a tile's last row, or a window's and what its tokens span
     c.limit = a.window > 0 ? min(q.n, min(a.window, q.n) + (tr - 1) / c.G + 1) : q.n;
     c.chunk = chunk;
-    c.nc = max(1, (int)(((long long)c.limit + chunk - 1) / chunk));
+    c.nc = max(1, (int)(((uint32_t)c.limit + (uint32_t)(chunk - 1)) / (uint32_t)chunk));
     c.c0 = q.p0 > 0 ? min(c.nc, q.p0 / chunk + 1) : 1;
     return c;
 }
@@ -434,10 +433,10 @@ struct Pieces {
 };
 template <bool THIN>
 __device__ __forceinline__ Pieces pieces_of(const Cut &c, int t) {
-    const long long rows = min((long long)(t + 1) * kTileRows<THIN>, (long long)c.rows);
-    const int span = max(0, min(c.p0 + (int)((rows + c.G - 1) / c.G), c.limit));
-    const int n = max(1, (int)(((long long)span + c.chunk - 1) / c.chunk));
-    return {n, (int)((((long long)span + n - 1) / n + 127) / 128 * 128)};
+    const uint32_t rows = min((uint32_t)(t + 1) * kTileRows<THIN>, (uint32_t)c.rows);
+    const uint32_t span = (uint32_t)max(0, min(c.p0 + (int)((rows + (uint32_t)c.G - 1) / (uint32_t)c.G), c.limit));
+    const uint32_t n = max(1u, (span + (uint32_t)(c.chunk - 1)) / (uint32_t)c.chunk);
+    return {(int)n, (int)(((span + n - 1) / n + 127) / 128 * 128)};
 }
 
 // Rows that a block of the merge launch joins: a few per wave, or where many pieces have to be read, as many as one
@@ -559,19 +558,26 @@ __device__ int schedule(const AttnArgs &a, int32_t *s_items, int32_t *s_units, S
     }
 }
 
-// Two f32 as packed bf16 by truncation, and what that leaves of them.
-__device__ __forceinline__ uint32_t take_part(float &x, float &y) {
-    const uint32_t ux = __float_as_uint(x), uy = __float_as_uint(y);
-    x -= __uint_as_float(ux & 0xFFFF0000u);
-    y -= __uint_as_float(uy & 0xFFFF0000u);
-    return __builtin_amdgcn_perm(uy, ux, 0x07060302u);
+// Two f32 as packed bf16, to nearest, and exactly what that leaves of them: x - hi(x) is one dot product of the pair with
+// (-1, 0) instead of an unpack and a subtraction (the weights' parts are a third of a step's arithmetic). The
+// constants stay in registers: as literals of the packed type the compiler encodes one of them as the other.
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+struct PartConsts {
+    uint32_t lo = 0x0000BF80u, hi = 0xBF800000u;
+    __device__ __forceinline__ PartConsts() { asm("" : "+v"(lo), "+v"(hi)); }
+};
+__device__ __forceinline__ uint32_t take_part(float &x, float &y, const PartConsts &pc) {
+    const bf16x2 h = {(__bf16)x, (__bf16)y};
+    x = __builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(bf16x2, pc.lo), x, false);
+    y = __builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(bf16x2, pc.hi), y, false);
+    return __builtin_bit_cast(uint32_t, h);
 }
 // Eight f32 in three parts.
-__device__ __forceinline__ void split3(float (&x)[8], u32x4 (&part)[3]) {
+__device__ __forceinline__ void split3(float (&x)[8], u32x4 (&part)[3], const PartConsts &pc) {
 #pragma unroll
     for (int p = 0; p < 3; ++p)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) part[p][i] = take_part(x[2 * i], x[2 * i + 1]);
+        for (int i = 0; i < 4; ++i) part[p][i] = take_part(x[2 * i], x[2 * i + 1], pc);
 }
 
 // max and sum over the four lanes of a query
@@ -624,19 +630,22 @@ struct SwizzledTile {
 
 extern __shared__ __align__(16) uint8_t smem[];
 
-// What a wave keeps of its NQ * 16 rows.
-template <int HDP, int NQ>
+// What a wave keeps of its NQ * 16 rows. QP: parts of the query rows in registers; the third may lie in LDS instead, from
+// q_at on for this lane, laid out as a PaddedTile of the wave's rows.
+template <int HDP, int NQ, int QP = 3>
 struct WaveState {
-    u32x4 q[NQ][HDP / 32][3];
+    u32x4 q[NQ][HDP / 32][QP];
+    int q_at;
     f32x4 o[NQ][HDP / 16];
     float m[NQ], l[NQ];
     int pos[NQ];  // this lane's query's position
+    PartConsts pc;
 };
 
 // 32 positions, staged from byte k_off (keys) and v_off (values) of LDS on, parts `part` bytes apart; between(i) is called among the products, for i = 0 .. HDP / 16 NP - 1 in turn; seen(n): bit 4 t + i, whether query n of this lane sees key 16 t + 4 g + i of them
 // (asked where !full).
-template <int HDP, int NQ, int NP, int part, typename Tile, typename Between, typename Seen>
-__device__ __forceinline__ void attn_step(WaveState<HDP, NQ> &w, const Tile &tile, int k_off, int v_off, bool full,
+template <int HDP, int NQ, int QP, int NP, int part, typename Tile, typename Between, typename Seen>
+__device__ __forceinline__ void attn_step(WaveState<HDP, NQ, QP> &w, const Tile &tile, int k_off, int v_off, bool full,
                                           Between between, Seen seen) {
     // Consecutive products go to different sums: a sum's next product waits for its last. The operands of the next
     // products are read from LDS before those of the last ones are used.
@@ -669,6 +678,11 @@ __device__ __forceinline__ void attn_step(WaveState<HDP, NQ> &w, const Tile &til
             read_k(i + 1, k[(i + 1) & 1]);
         else
             read_v(0, v[0]);
+        u32x4 q3[NQ];
+        if (QP < 3 && i % NP == 0)
+#pragma unroll
+            for (int n = 0; n < NQ; ++n)
+                q3[n] = *reinterpret_cast<const u32x4 *>(smem + w.q_at + n * 16 * PaddedTile<HDP>::ROW + i / NP * 64);
         between(i);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -676,7 +690,8 @@ __device__ __forceinline__ void attn_step(WaveState<HDP, NQ> &w, const Tile &til
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int n = 0; n < NQ; ++n) s[n][t] = mfma(k[i & 1][t], w.q[n][i / NP][qp], s[n][t]);
+                for (int n = 0; n < NQ; ++n)
+                    s[n][t] = mfma(k[i & 1][t], qp < QP ? w.q[n][i / NP][qp < QP ? qp : 0] : q3[n], s[n][t]);
         __builtin_amdgcn_sched_barrier(0);
     }
     if (!full) {
@@ -725,7 +740,7 @@ __device__ __forceinline__ void attn_step(WaveState<HDP, NQ> &w, const Tile &til
                 e[4 * t + i] = __builtin_amdgcn_exp2f(s[n][t][i] - ref);
                 w.l[n] += e[4 * t + i];
             }
-        split3(e, p[n]);
+        split3(e, p[n], w.pc);
     }
 #pragma unroll
     for (int i = 0; i < VI; ++i) {
@@ -746,15 +761,15 @@ __device__ __forceinline__ void attn_step(WaveState<HDP, NQ> &w, const Tile &til
 }
 
 // The rows of a wave: rows row0 .. row0 + 16 NQ - 1 of the request (clamped to its last), q in three parts.
-template <int HDP, int NQ>
-__device__ __forceinline__ void wave_init(WaveState<HDP, NQ> &w, const AttnArgs &a, const Request &q, int rows, int kvh,
-                                          int row0) {
+template <int HDP, int NQ, int QP>
+__device__ __forceinline__ void wave_init(WaveState<HDP, NQ, QP> &w, const AttnArgs &a, const Request &q, int rows, int kvh,
+                                          int row0, int q_off) {
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, G = (int)a.group.d;
+    w.q_at = q_off + c * PaddedTile<HDP>::ROW + 16 * g;
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
         const int row = min(row0 + 16 * n + c, rows - 1), tok = (int)page_of((uint32_t)row, a.group);
-        const int h = kvh * G + row - tok * G;
-        const float *src = a.q + (size_t)(q.t0 + tok) * a.q_stride + (size_t)h * a.d.hd + 8 * g;
+        const float *src = a.q + (size_t)(q.t0 + tok) * a.q_stride + (size_t)(kvh * G + row - tok * G) * a.d.hd + 8 * g;
         w.pos[n] = q.p0 + tok;
         w.m[n] = -INFINITY;
         w.l[n] = 0.0f;
@@ -769,33 +784,50 @@ __device__ __forceinline__ void wave_init(WaveState<HDP, NQ> &w, const AttnArgs 
                 x[i] = x0[i] * a.scale2;
                 x[4 + i] = x1[i] * a.scale2;
             }
-            split3(x, w.q[n][st]);
+            u32x4 part[3];
+            split3(x, part, w.pc);
+#pragma unroll
+            for (int p = 0; p < QP; ++p) w.q[n][st][p] = part[p];
+            if (QP < 3)
+                *reinterpret_cast<u32x4 *>(smem + w.q_at + n * 16 * PaddedTile<HDP>::ROW + st * 64) = part[2];
         }
 #pragma unroll
         for (int d = 0; d < HDP / 16; ++d) w.o[n][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 }
 
-// The places (byte offset of the block) of the pages that positions j0 .. j1 - 1 (at most tab_span of them) lie on, into
-// s_tab; 1 for a page outside the cache (whose positions are read from offset 0 and not seen): whether there is any.
-// For all threads of the block.
+// The places (byte offset of the block) of the pages that positions j0 .. j1 - 1 (at most tab_span of them, at least
+// one) lie on: ask() for the block numbers, fill() s_tab; 1 for a page outside the cache (whose positions are read
+// from offset 0 and not seen): whether there is any. For all threads of the block.
 constexpr int kTabBytes = 8 * kTabPages;
 __device__ __forceinline__ int tab_span(const AttnArgs &a) {
     return (int)(min((kTabPages - 1) * (long long)a.d.block_size, (long long)kMaxChunk) / 128 * 128);
 }
 template <int DT>
-__device__ __forceinline__ bool fill_tab(const AttnArgs &a, int r, int j0, int j1, uint64_t *s_tab) {
-    const int page0 = (int)page_of((uint32_t)j0, a.d.div), n = (int)page_of((uint32_t)(j1 - 1), a.d.div) - page0 + 1;
-    bool bad = false;
-    __syncthreads();  // the last table has been read
-    for (int i = threadIdx.x; i < n; i += 256) {
-        const int b = a.tables[(size_t)r * a.max_blocks + page0 + i];
-        const bool ok = b >= 0 && b < a.d.n_blocks;
-        bad |= !ok;
-        s_tab[i] = ok ? (uint64_t)b * a.d.block_stride * (DT == RBT_DT_BF16 ? 2 : 4) : 1;
+struct PageTab {
+    int b[(kTabPages + 255) / 256], n;
+    __device__ __forceinline__ void ask(const AttnArgs &a, int r, int j0, int j1) {
+        const int page0 = (int)page_of((uint32_t)j0, a.d.div);
+        n = (int)page_of((uint32_t)(j1 - 1), a.d.div) - page0 + 1;
+#pragma unroll
+        for (int i = 0; i < (kTabPages + 255) / 256; ++i) {
+            const int p = (int)threadIdx.x + 256 * i;
+            b[i] = p < n ? a.tables[(size_t)r * a.max_blocks + page0 + p] : 0;
+        }
     }
-    return __builtin_amdgcn_readfirstlane(__syncthreads_or(bad)) != 0;
-}
+    __device__ __forceinline__ bool fill(const AttnArgs &a, uint64_t *s_tab) const {
+        bool bad = false;
+        __syncthreads();  // the last table has been read
+#pragma unroll
+        for (int i = 0; i < (kTabPages + 255) / 256; ++i) {
+            const int p = (int)threadIdx.x + 256 * i;
+            const bool ok = b[i] >= 0 && b[i] < a.d.n_blocks;
+            bad |= p < n && !ok;
+            if (p < n) s_tab[p] = ok ? (uint64_t)b[i] * a.d.block_stride * (DT == RBT_DT_BF16 ? 2 : 4) : 1;
+        }
+        return __builtin_amdgcn_readfirstlane(__syncthreads_or(bad)) != 0;
+    }
+};
 // Where a position's row of a head (head_off: the head's bytes in a block) lies in the cache.
 template <int DT>
 __device__ __forceinline__ uint64_t row_at(const AttnArgs &a, const uint64_t *s_tab, int page0, uint32_t head_off, int pos) {
@@ -821,6 +853,7 @@ struct Stage {
     static constexpr int LD = DT == RBT_DT_BF16 ? 1 : 2;
     static_assert(N * ROWS == KEYS, "whole passes");
     u32x4 k[N][LD], v[N][LD];
+    PartConsts pc;
 
     __device__ __forceinline__ void load(const AttnArgs &a, const uint64_t *s_tab, int page0, int kvh, int j, int last,
                                          int tid) {
@@ -849,7 +882,7 @@ struct Stage {
             u32x4 p[3];
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(r[i / 4][i % 4]);
-            split3(x, p);
+            split3(x, p, pc);
 #pragma unroll
             for (int y = 0; y < 3; ++y) *reinterpret_cast<u32x4 *>(smem + off + y * part) = p[y];
         }
@@ -865,32 +898,40 @@ struct Stage {
     }
 };
 
-// The same for a bf16 tile of a block's four waves as direct copies into LDS (SwizzledTile), not waited for: aim() finds
-// the places, copy(i) makes the i-th of a wave's COPIES. A copy holds up its wave while the ones before it are taken
-// (32 KiB at 64 bytes a clock), so they are made one by one among the products of the tile before. A head dim below HDP:
-// the chunks behind it repeat its last (the query's are 0, and the output's are not stored).
+// The same for a bf16 tile of a block's four waves as direct copies into LDS (SwizzledTile), not waited for. A head dim
+// below HDP: the chunks behind it repeat its last (the query's are 0, and the output's are not stored).
 template <int HDP, int KEYS>
 struct TileCopy {
     using Tile = SwizzledTile<HDP>;
-    static constexpr int ROWS = 64 / Tile::CH, N = KEYS / 4 / ROWS, COPIES = 2 * N;  // rows per copy
+    static constexpr int ROWS = 64 / Tile::CH, N = KEYS / 4 / ROWS;  // rows per copy
     static_assert(N * 4 * ROWS == KEYS, "whole copies");
     uint64_t at[N];
-    uint32_t lds;
-    __device__ __forceinline__ void aim(const AttnArgs &a, const uint64_t *s_tab, int page0, int kvh, int j, int last,
-                                        int buf) {
+    uint32_t lds0, in[N];
+    __device__ __forceinline__ TileCopy() {
+        const int wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+        lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)smem + (uint32_t)(wv * N * ROWS * Tile::ROW);
+    }
+    // The places of the tile from position j on, in two steps: the table is asked, its answers used.
+    __device__ __forceinline__ void look(const AttnArgs &a, const uint64_t *s_tab, int page0, uint32_t head_off, int j,
+                                         int last) {
         const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-        const uint32_t head_off = head_offset<RBT_DT_BF16>(a, kvh);
-        lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)smem + (uint32_t)(buf + wv * N * ROWS * Tile::ROW);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int row = (wv * N + i) * ROWS + lane / Tile::CH;
-            const int chunk = min((lane % Tile::CH) ^ Tile::key(row), a.d.hd / 8 - 1);
-            at[i] = row_at<RBT_DT_BF16>(a, s_tab, page0, head_off, min(j + row, last)) + 16 * chunk;
+            const int row = (wv * N + i) * ROWS + lane / Tile::CH, pos = min(j + row, last);
+            const int chunk = min((lane % Tile::CH) ^ Tile::key(row), a.d.hd / 8 - 1), page = (int)page_of((uint32_t)pos, a.d.div);
+            in[i] = head_off + (uint32_t)(pos - page * a.d.block_size) * (uint32_t)(2 * a.d.hd) + 16u * (uint32_t)chunk;
+            at[i] = s_tab[page - page0];
         }
     }
-    __device__ __forceinline__ void copy(const AttnArgs &a, int i) const {
-        const uint8_t *src = static_cast<const uint8_t *>(i & 1 ? a.vc : a.kc);
-        lds_dma16(src + at[i / 2], lds + (uint32_t)(((i & 1) * KEYS + i / 2 * ROWS) * Tile::ROW));
+    __device__ __forceinline__ void aim() {
+#pragma unroll
+        for (int i = 0; i < N; ++i) at[i] = (at[i] & ~(uint64_t)15) + in[i];
+    }
+    __device__ __forceinline__ void copies(const AttnArgs &a, int buf) const {
+#pragma unroll
+        for (int i = 0; i < 2 * N; ++i)
+            lds_dma16(static_cast<const uint8_t *>(i & 1 ? a.vc : a.kc) + at[i / 2],
+                      lds0 + (uint32_t)(buf + ((i & 1) * KEYS + i / 2 * ROWS) * Tile::ROW));
     }
 };
 
@@ -1061,11 +1102,14 @@ __global__ __launch_bounds__(256, (ThinShape<HDP>::PER_CU)) void attn_thin_kerne
         const Item x = item_of<true, HDP>(a, items.it, chunk, s_items, s_units);
         const int ticket = items.ask();
         WaveState<HDP, 1> w;
-        wave_init<HDP, 1>(w, a, x.q, x.cut.rows, x.kvh, x.row0);
+        PageTab<DT> tab;
+        if (x.k0 < x.k1) tab.ask(a, x.r, x.k0, x.k0 + min(span, x.k1 - x.k0));
+        wave_init(w, a, x.q, x.cut.rows, x.kvh, x.row0, 0);
         const int k_off = wv * WAVE, v_off = k_off + 32 * PaddedTile<HDP>::ROW;
         for (int w0 = x.k0; w0 < x.k1; w0 += span) {
             const int w1 = min(x.k1, w0 + min(span, x.k1 - w0)), page0 = (int)page_of((uint32_t)w0, a.d.div);
-            const bool bad = fill_tab<DT>(a, x.r, w0, w1, s_tab);
+            if (w0 != x.k0) tab.ask(a, x.r, w0, w1);
+            const bool bad = tab.fill(a, s_tab);
             Stage<DT, HDP, 32, 64, true> st;
             int j = w0 + 32 * wv;
             if (j < w1) st.load(a, s_tab, page0, x.kvh, j, w1 - 1, lane);
@@ -1075,7 +1119,7 @@ __global__ __launch_bounds__(256, (ThinShape<HDP>::PER_CU)) void attn_thin_kerne
                 __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
                 if (j + 128 < w1) st.load(a, s_tab, page0, x.kvh, j + 128, w1 - 1, lane);
                 const bool full = !bad && j + 32 <= min(w1, x.pa + 1) && (a.window <= 0 || j > x.pb - a.window);
-                attn_step<HDP, 1, 1, 0>(w, tl, k_off, v_off, full, [](int) {},
+                attn_step<HDP, 1, 3, 1, 0>(w, tl, k_off, v_off, full, [](int) {},
                                         [&](int n) { return seen_bits(a, j, w1, w.pos[n], s_tab, page0, bad); });
             }
         }
@@ -1140,13 +1184,13 @@ __global__ __launch_bounds__(256, (ThinShape<HDP>::PER_CU)) void attn_thin_kerne
 template <int DT, int HDP>
 struct WideShape {
     static constexpr int NP = DT == RBT_DT_BF16 ? 1 : 3;
-    static constexpr int KEYS = 32;
     // bf16: two buffers that direct copies fill in turn; f32: one of parts, through registers
     static constexpr bool COPY = DT == RBT_DT_BF16;
     using Tile = std::conditional_t<COPY, SwizzledTile<HDP>, PaddedTile<HDP>>;
-    static_assert(COPY || KEYS == 32, "a tile of parts is one step");
-    static constexpr int PART = KEYS * Tile::ROW, BUF = 2 * NP * PART;
-    static constexpr int TILE = COPY ? 2 * BUF : BUF;
+    static constexpr int PART = 32 * Tile::ROW, BUF = 2 * NP * PART;
+    // with two blocks to a CU there are registers for two of the query rows' three parts
+    static constexpr int QP = COPY && HDP == 128 ? 2 : 3, Q_AT = COPY ? 2 * BUF : BUF;
+    static constexpr int TILE = Q_AT + (QP < 3 ? kWideRows * PaddedTile<HDP>::ROW : 0);
     static constexpr int PER_CU = HDP <= 128 ? 2 : 1;
     static_assert(sizeof(RowShared) <= (size_t)TILE, "row_any's LDS");
 };
@@ -1170,49 +1214,57 @@ __global__ __launch_bounds__(256, (WideShape<DT, HDP>::PER_CU)) void attn_wide_k
         const bool active = 32 * wv < x.n_rows;
         const int wa = place(a, x.q, x.kvh, min(wr0, x.cut.rows - 1)).pos,
                   wb = place(a, x.q, x.kvh, min(wr0 + 31, x.cut.rows - 1)).pos;
-        WaveState<HDP, 2> w;
-        wave_init<HDP, 2>(w, a, x.q, x.cut.rows, x.kvh, wr0);
+        WaveState<HDP, 2, Sh::QP> w;
+        PageTab<DT> tab;
+        if (x.k0 < x.k1) tab.ask(a, x.r, x.k0, x.k0 + min(span, x.k1 - x.k0));
+        wave_init(w, a, x.q, x.cut.rows, x.kvh, wr0, Sh::Q_AT + 32 * wv * PaddedTile<HDP>::ROW);
         for (int w0 = x.k0; w0 < x.k1; w0 += span) {
             const int w1 = min(x.k1, w0 + min(span, x.k1 - w0)), page0 = (int)page_of((uint32_t)w0, a.d.div);
-            const bool bad = fill_tab<DT>(a, x.r, w0, w1, s_tab);
+            if (w0 != x.k0) tab.ask(a, x.r, w0, w1);
+            const bool bad = tab.fill(a, s_tab);
             // the wave's part of 32 staged positions from j on: whether it has any
             auto step = [&](int j, int off, auto between) {
                 if (!active || j >= w1 || j > wb || (a.window > 0 && j + 31 <= wa - a.window)) return false;
                 const bool full = !bad && j + 32 <= min(w1, wa + 1) && (a.window <= 0 || j > wb - a.window);
-                attn_step<HDP, 2, Sh::NP, Sh::PART>(
+                attn_step<HDP, 2, Sh::QP, Sh::NP, Sh::PART>(
                     w, tl, off, off + Sh::NP * Sh::PART, full, between,
                     [&](int n) { return seen_bits(a, j, w1, w.pos[n], s_tab, page0, bad); });
                 return true;
             };
             if constexpr (Sh::COPY) {
-                TileCopy<HDP, Sh::KEYS> cp;
-                static_assert(cp.COPIES <= HDP / 16, "a step has room for a tile's copies");
-                auto copies = [&]() {
-#pragma unroll
-                    for (int i = 0; i < cp.COPIES; ++i) cp.copy(a, i);
-                };
-                cp.aim(a, s_tab, page0, x.kvh, w0, w1 - 1, 0);
-                copies();
+                // A tile's copies are made a step ahead, and the places of the tile after it are looked up
+                // among the products of that step.
+                TileCopy<HDP, 32> cp;
+                const uint32_t head_off = head_offset<DT>(a, x.kvh);
+                auto look = [&](int j) { cp.look(a, s_tab, page0, head_off, j, w1 - 1); };
+                look(w0);
+                cp.aim();
+                cp.copies(a, 0);
+                look(w0 + 32);
+                cp.aim();
                 int buf = 0;
-                for (int jt = w0; jt < w1; jt += Sh::KEYS) {
+                for (int j = w0; j < w1; j += 32) {
                     wait_dma<0>();
                     __syncthreads();  // this tile has landed for all, and the last one has been read
-                    const bool more = jt + Sh::KEYS < w1;
-                    if (more) cp.aim(a, s_tab, page0, x.kvh, jt + Sh::KEYS, w1 - 1, buf ^ Sh::BUF);
-                    if (more) copies();
-                    step(jt, buf, [](int) {});
-#pragma unroll
-                    for (int u = 32; u < Sh::KEYS; u += 32) step(jt + u, buf + u * Sh::Tile::ROW, [](int) {});
+                    if (j + 32 < w1) cp.copies(a, buf ^ Sh::BUF);
+                    const bool done = step(j, buf, [&](int i) {
+                        if (i == 0) look(j + 64);
+                        if (i == 2) cp.aim();
+                    });
+                    if (!done) {
+                        look(j + 64);
+                        cp.aim();
+                    }
                     buf ^= Sh::BUF;
                 }
             } else {
-                Stage<DT, HDP, Sh::KEYS, 256, false> st;
+                Stage<DT, HDP, 32, 256, false> st;
                 st.load(a, s_tab, page0, x.kvh, w0, w1 - 1, tid);
-                for (int jt = w0; jt < w1; jt += Sh::KEYS) {
+                for (int jt = w0; jt < w1; jt += 32) {
                     __syncthreads();
                     st.store(0, Sh::NP * Sh::PART, Sh::PART, tid);
                     __syncthreads();
-                    if (jt + Sh::KEYS < w1) st.load(a, s_tab, page0, x.kvh, jt + Sh::KEYS, w1 - 1, tid);
+                    if (jt + 32 < w1) st.load(a, s_tab, page0, x.kvh, jt + 32, w1 - 1, tid);
                     step(jt, 0, [](int) {});
                 }
             }
