@@ -769,20 +769,21 @@ __device__ __forceinline__ void wave_init(WaveState<HDP, NQ, QP> &w, const AttnA
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
         const int row = min(row0 + 16 * n + c, rows - 1), tok = (int)page_of((uint32_t)row, a.group);
-        const float *src = a.q + (size_t)(q.t0 + tok) * a.q_stride + (size_t)(kvh * G + row - tok * G) * a.d.hd + 8 * g;
+        const float *src = a.q + (size_t)(q.t0 + tok) * a.q_stride + (size_t)(kvh * G + row - tok * G) * a.d.hd;
         w.pos[n] = q.p0 + tok;
         w.m[n] = -INFINITY;
         w.l[n] = 0.0f;
 #pragma unroll
         for (int st = 0; st < HDP / 32; ++st) {
             float x[8];
-            const bool in = 32 * st + 8 * g < a.d.hd;
-            const f32x4 x0 = in ? ld_f4(src + 32 * st) : f32x4{0.0f, 0.0f, 0.0f, 0.0f},
-                        x1 = in ? ld_f4(src + 32 * st + 4) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            // past the head's end: its last 8 elements, as 0 (a branch here would make each load wait for the one before)
+            const int at = min(32 * st + 8 * g, a.d.hd - 8);
+            const f32x4 x0 = ld_f4(src + at), x1 = ld_f4(src + at + 4);
+            const float scale = at == 32 * st + 8 * g ? a.scale2 : 0.0f;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                x[i] = x0[i] * a.scale2;
-                x[4 + i] = x1[i] * a.scale2;
+                x[i] = x0[i] * scale;
+                x[4 + i] = x1[i] * scale;
             }
             u32x4 part[3];
             split3(x, part, w.pc);
@@ -857,20 +858,16 @@ struct Stage {
 
     __device__ __forceinline__ void load(const AttnArgs &a, const uint64_t *s_tab, int page0, int kvh, int j, int last,
                                          int tid) {
-        const int row = tid / CH, chunk = tid % CH;
+        const int row = tid / CH, chunk = min(tid % CH, a.d.hd / 8 - 1);  // behind the head's end: its last chunk
         const uint32_t head_off = head_offset<DT>(a, kvh);
-        const bool in = 8 * chunk < a.d.hd;
         constexpr size_t esz = DT == RBT_DT_BF16 ? 2 : 4;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const uint64_t at = row_at<DT>(a, s_tab, page0, head_off, min(j + row + i * ROWS, last)) + 8 * chunk * esz;
 #pragma unroll
             for (int x = 0; x < LD; ++x) {
-                k[i][x] = v[i][x] = u32x4{0, 0, 0, 0};
-                if (in) {
-                    k[i][x] = ld_kv<ONCE>(static_cast<const uint8_t *>(a.kc) + at + 16 * x);
-                    v[i][x] = ld_kv<ONCE>(static_cast<const uint8_t *>(a.vc) + at + 16 * x);
-                }
+                k[i][x] = ld_kv<ONCE>(static_cast<const uint8_t *>(a.kc) + at + 16 * x);
+                v[i][x] = ld_kv<ONCE>(static_cast<const uint8_t *>(a.vc) + at + 16 * x);
             }
         }
     }
