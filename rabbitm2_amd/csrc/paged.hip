@@ -353,7 +353,7 @@ __global__ __launch_bounds__(256) void attn_any_kernel(AttnArgs a) {
 // Rows: a request's new tokens times the query heads of one key/value head, heads fastest. A tile of rows runs over
 // its positions in tiles, staged in LDS as bf16 parts:
 //   wide   128 rows, 32 to a wave; the block's waves share each tile of keys and values
-//   thin   requests of up to 16 rows (a decoding token) on a bf16 cache: each wave takes tiles of 32 positions
+//   thin   requests of up to 16 rows (a decoding token): each wave takes tiles of 32 positions of its own
 // in two launches, and long ranges are cut into chunks that different blocks take, joined by a third.
 //
 // Products: v_mfma_f32_16x16x32_bf16, transposed so that nothing moves between lanes: S^T = K Q^T leaves lane
@@ -1072,22 +1072,112 @@ __device__ __forceinline__ void again_rows(const AttnArgs &a, const Item &x, con
 constexpr int kLdsBytes = 159 << 10;  // of 160 KiB: the kernels' fixed shared variables take less than the last
 constexpr int attn_lds(int tile, int n_req) { return tile + kTabBytes + 8 * (n_req + 1); }
 
-// Requests of up to 16 rows.
+// A thin wave on an f32 cache: v_mfma_f32_16x16x4_f32 on f32 operands straight from the cache, 16 positions at a time (a
+// decoding row reads every key once: its products wait for memory whichever unit makes them, and nothing has to be
+// taken apart). The layout is the bf16 one's with steps of four: S^T leaves lane (c, g) the keys 4 g + i of query c,
+// the B operands of four steps of O^T = V^T P^T. K enters 16 bytes per lane (key c, dims 16 s + 4 g + i), V too (key
+// 4 g + i, dims 64 h + 4 c + d).
 template <int HDP>
+struct ThinF32 {
+    f32x4 q[HDP / 16], o[HDP / 64][4];  // o[h][d][i]: dim 64 h + 4 (4 g + i) + d
+    float m, l;
+    int pos;
+    f32x4 k[HDP / 16], v[4][HDP / 64];  // the positions at hand; the next ones' are asked for as soon as each is used
+    __device__ __forceinline__ void init(const AttnArgs &a, const Item &x) {
+        const int c = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
+        const Place pl = place(a, x.q, x.kvh, min(x.row0 + c, x.cut.rows - 1));
+        const float *src = a.q + (size_t)pl.t * a.q_stride + (size_t)pl.h * a.d.hd;
+        pos = pl.pos;
+        m = -INFINITY;
+        l = 0.0f;
+#pragma unroll
+        for (int s = 0; s < HDP / 16; ++s) {
+            const int at = min(16 * s + 4 * g, a.d.hd - 4);
+            q[s] = ld_f4(src + at) * (at == 16 * s + 4 * g ? a.scale2 : 0.0f);
+        }
+#pragma unroll
+        for (int h = 0; h < HDP / 64; ++h)
+#pragma unroll
+            for (int d = 0; d < 4; ++d) o[h][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    __device__ __forceinline__ void load_k(const AttnArgs &a, const uint64_t *s_tab, int page0, uint32_t head_off, int j,
+                                           int last) {
+        const int c = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
+        const uint8_t *p = static_cast<const uint8_t *>(a.kc) + row_at<RBT_DT_F32>(a, s_tab, page0, head_off, min(j + c, last));
+#pragma unroll
+        for (int s = 0; s < HDP / 16; ++s) k[s] = ld_stream_f4(p + 4 * min(16 * s + 4 * g, a.d.hd - 4));
+    }
+    __device__ __forceinline__ void load_v(const AttnArgs &a, const uint64_t *s_tab, int page0, uint32_t head_off, int j,
+                                           int last) {
+        const int c = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint8_t *p = static_cast<const uint8_t *>(a.vc) +
+                               row_at<RBT_DT_F32>(a, s_tab, page0, head_off, min(j + 4 * g + i, last));
+#pragma unroll
+            for (int h = 0; h < HDP / 64; ++h) v[i][h] = ld_stream_f4(p + 4 * min(64 * h + 4 * c, a.d.hd - 4));
+        }
+    }
+    // seen(): bit i, whether the lane's query sees key 4 g + i; then_k, then_v: called when the keys, the values
+    // have been used
+    template <typename Seen, typename ThenK, typename ThenV>
+    __device__ __forceinline__ void step(bool full, Seen seen, ThenK then_k, ThenV then_v) {
+        f32x4 s2[2] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}, f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+        for (int s = 0; s < HDP / 16; ++s)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s2[i & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s][i], q[s][i], s2[i & 1], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        then_k();
+        f32x4 s = s2[0] + s2[1];
+        if (!full) {
+            const uint32_t bits = seen();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[i] = bits >> i & 1 ? s[i] : -INFINITY;
+        }
+        const float top = fmaxf(fmaxf(s.x, s.y), fmaxf(s.z, s.w));
+        if (__any(top > m + 8.0f)) {  // as attn_step's
+            const float mx = fmaxf(m, group_max(top)), f = m == -INFINITY ? 0.0f : exp2f(m - mx);
+            m = mx;
+            l *= f;
+#pragma unroll
+            for (int h = 0; h < HDP / 64; ++h)
+#pragma unroll
+                for (int d = 0; d < 4; ++d) o[h][d] *= f;
+        }
+        const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float p = __builtin_amdgcn_exp2f(s[i] - ref);
+            l += p;
+#pragma unroll
+            for (int h = 0; h < HDP / 64; ++h)
+#pragma unroll
+                for (int d = 0; d < 4; ++d)
+                    o[h][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i][h][d], p, o[h][d], 0, 0, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        then_v();
+    }
+};
+
+// Requests of up to 16 rows.
+template <int DT, int HDP>
 struct ThinShape {
-    static constexpr int WAVE = 2 * 32 * PaddedTile<HDP>::ROW;  // a wave's own keys and values, and later its rows
+    static constexpr int ROWS = kThinRows * (HDP + 4) * 4;  // a wave's rows, when the waves' states are joined
+    static constexpr int WAVE = DT == RBT_DT_BF16 ? 2 * 32 * PaddedTile<HDP>::ROW : ROWS;  // bf16: keys and values before
     static constexpr int TILE = 4 * WAVE;
     static constexpr int PER_CU = HDP <= 128 ? 2 : 1;  // blocks that share a CU
-    static_assert(kThinRows * (HDP + 4) * 4 <= WAVE, "a wave's rows fit its tile");
+    static_assert(ROWS <= WAVE, "a wave's rows fit its tile");
     static_assert(sizeof(RowShared) <= (size_t)TILE, "row_any's LDS");
 };
-template <int HDP>
-__global__ __launch_bounds__(256, (ThinShape<HDP>::PER_CU)) void attn_thin_kernel(AttnArgs a) {
-    constexpr int DT = RBT_DT_BF16, WAVE = ThinShape<HDP>::WAVE;
+template <int DT, int HDP>
+__global__ __launch_bounds__(256, (ThinShape<DT, HDP>::PER_CU)) void attn_thin_kernel(AttnArgs a) {
+    constexpr int WAVE = ThinShape<DT, HDP>::WAVE;
     __shared__ ScheduleShared s_sched;
     __shared__ float s_m[4][kThinRows], s_l[4][kThinRows];
     __shared__ int s_flag[kThinRows], s_next;
-    uint64_t *s_tab = reinterpret_cast<uint64_t *>(smem + ThinShape<HDP>::TILE);
+    uint64_t *s_tab = reinterpret_cast<uint64_t *>(smem + ThinShape<DT, HDP>::TILE);
     int32_t *s_items = reinterpret_cast<int32_t *>(s_tab + kTabPages), *s_units = s_items + a.n_req + 1;
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
     const int chunk = __builtin_amdgcn_readfirstlane(schedule<true, HDP>(a, s_items, s_units, s_sched));
@@ -1098,38 +1188,75 @@ __global__ __launch_bounds__(256, (ThinShape<HDP>::PER_CU)) void attn_thin_kerne
     while (items.it >= 0) {
         const Item x = item_of<true, HDP>(a, items.it, chunk, s_items, s_units);
         const int ticket = items.ask();
-        WaveState<HDP, 1> w;
         PageTab<DT> tab;
         if (x.k0 < x.k1) tab.ask(a, x.r, x.k0, x.k0 + min(span, x.k1 - x.k0));
-        wave_init(w, a, x.q, x.cut.rows, x.kvh, x.row0, 0);
-        const int k_off = wv * WAVE, v_off = k_off + 32 * PaddedTile<HDP>::ROW;
-        for (int w0 = x.k0; w0 < x.k1; w0 += span) {
-            const int w1 = min(x.k1, w0 + min(span, x.k1 - w0)), page0 = (int)page_of((uint32_t)w0, a.d.div);
-            if (w0 != x.k0) tab.ask(a, x.r, w0, w1);
-            const bool bad = tab.fill(a, s_tab);
-            Stage<DT, HDP, 32, 64, true> st;
-            int j = w0 + 32 * wv;
-            if (j < w1) st.load(a, s_tab, page0, x.kvh, j, w1 - 1, lane);
-            for (; j < w1; j += 128) {
-                __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
-                st.store(k_off, v_off, 0, lane);
-                __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
-                if (j + 128 < w1) st.load(a, s_tab, page0, x.kvh, j + 128, w1 - 1, lane);
-                const bool full = !bad && j + 32 <= min(w1, x.pa + 1) && (a.window <= 0 || j > x.pb - a.window);
-                attn_step<HDP, 1, 3, 1, 0>(w, tl, k_off, v_off, full, [](int) {},
-                                        [&](int n) { return seen_bits(a, j, w1, w.pos[n], s_tab, page0, bad); });
+        // fn(w0, w1, page0, bad) over the stretches of the piece that the table holds
+        auto stretches = [&](auto fn) {
+            for (int w0 = x.k0; w0 < x.k1; w0 += span) {
+                const int w1 = min(x.k1, w0 + min(span, x.k1 - w0));
+                if (w0 != x.k0) tab.ask(a, x.r, w0, w1);
+                const bool bad = tab.fill(a, s_tab);
+                fn(w0, w1, (int)page_of((uint32_t)w0, a.d.div), bad);
             }
-        }
-        // the four waves' states, joined; each wave's rows lie where its tile was
-        w.l[0] = group_sum(w.l[0]);
-        if (g == 0) {
-            s_m[wv][c] = w.m[0];
-            s_l[wv][c] = w.l[0];
-        }
-        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+        };
+        auto whole = [&](int j, int n, int w1, bool bad) {  // whether all rows see all of n positions from j on
+            return !bad && j + n <= min(w1, x.pa + 1) && (a.window <= 0 || j > x.pb - a.window);
+        };
+        const int at = wv * WAVE;
+        // each wave's state, and its rows where its tile was
+        if constexpr (DT == RBT_DT_BF16) {
+            WaveState<HDP, 1> w;
+            wave_init(w, a, x.q, x.cut.rows, x.kvh, x.row0, 0);
+            const int v_off = at + 32 * PaddedTile<HDP>::ROW;
+            stretches([&](int w0, int w1, int page0, bool bad) {
+                Stage<DT, HDP, 32, 64, true> st;
+                int j = w0 + 32 * wv;
+                if (j < w1) st.load(a, s_tab, page0, x.kvh, j, w1 - 1, lane);
+                for (; j < w1; j += 128) {
+                    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+                    st.store(at, v_off, 0, lane);
+                    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+                    if (j + 128 < w1) st.load(a, s_tab, page0, x.kvh, j + 128, w1 - 1, lane);
+                    attn_step<HDP, 1, 3, 1, 0>(w, tl, at, v_off, whole(j, 32, w1, bad), [](int) {},
+                                               [&](int n) { return seen_bits(a, j, w1, w.pos[n], s_tab, page0, bad); });
+                }
+            });
+            w.l[0] = group_sum(w.l[0]);
+            if (g == 0) {
+                s_m[wv][c] = w.m[0];
+                s_l[wv][c] = w.l[0];
+            }
+            __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
 #pragma unroll
-        for (int d = 0; d < HDP / 16; ++d)
-            *reinterpret_cast<f32x4 *>(smem + k_off + (c * (HDP + 4) + 16 * d + 4 * g) * 4) = w.o[0][d];
+            for (int d = 0; d < HDP / 16; ++d)
+                *reinterpret_cast<f32x4 *>(smem + at + (c * (HDP + 4) + 16 * d + 4 * g) * 4) = w.o[0][d];
+        } else {
+            ThinF32<HDP> w;
+            w.init(a, x);
+            const uint32_t head_off = head_offset<DT>(a, x.kvh);
+            stretches([&](int w0, int w1, int page0, bool bad) {
+                int j = w0 + 16 * wv;
+                if (j < w1) {
+                    w.load_k(a, s_tab, page0, head_off, j, w1 - 1);
+                    w.load_v(a, s_tab, page0, head_off, j, w1 - 1);
+                }
+                for (; j < w1; j += 64)
+                    w.step(whole(j, 16, w1, bad), [&]() { return seen_bits(a, j, w1, w.pos, s_tab, page0, bad); },
+                           [&]() { if (j + 64 < w1) w.load_k(a, s_tab, page0, head_off, j + 64, w1 - 1); },
+                           [&]() { if (j + 64 < w1) w.load_v(a, s_tab, page0, head_off, j + 64, w1 - 1); });
+            });
+            w.l = group_sum(w.l);
+            if (g == 0) {
+                s_m[wv][c] = w.m;
+                s_l[wv][c] = w.l;
+            }
+#pragma unroll
+            for (int h = 0; h < HDP / 64; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<f32x4 *>(smem + at + (c * (HDP + 4) + 64 * h + 16 * g + 4 * i) * 4) =
+                        f32x4{w.o[h][0][i], w.o[h][1][i], w.o[h][2][i], w.o[h][3][i]};
+        }
         if (tid < kThinRows) s_flag[tid] = 0;
         __syncthreads();
         const int row = tid >> 4, y = tid & 15;
@@ -1479,10 +1606,11 @@ template <int DT, int HDP>
 hipError_t launch_attn(const Launch &L, const Launch &Lm, AttnArgs a) {
     using W = WideShape<DT, HDP>;
     const int G = a.n_heads / a.d.n_kv;
-    // Requests of up to 16 rows have a launch of their own on a bf16 cache, where its tiles and the step's prefix
-    // sums fit LDS (head dims above 128: up to 2900 requests). A launch that no request can belong to is left out;
+    // Requests of up to 16 rows have a launch of their own, where its tiles and the step's prefix sums fit LDS (a bf16
+    // cache with head dims above 128: up to 2900 requests). A launch that no request can belong to is left out;
     // otherwise each finds its requests on the device.
-    a.thin = DT == RBT_DT_BF16 && G <= kThinRows && attn_lds(ThinShape<HDP>::TILE, a.n_req) <= kLdsBytes;
+    using Th = ThinShape<DT, HDP>;
+    a.thin = G <= kThinRows && attn_lds(Th::TILE, a.n_req) <= kLdsBytes;
     const bool wide = !a.thin || (int64_t)a.T * G > kThinRows;
     static std::atomic<uint64_t> asked_w{0}, asked_t{0};
     hipError_t e = hipSuccess;
@@ -1493,12 +1621,11 @@ hipError_t launch_attn(const Launch &L, const Launch &Lm, AttnArgs a) {
             e = launch(a.thin ? Lm : L, attn_wide_kernel<DT, HDP>, dim3(256 * W::PER_CU), dim3(256),
                        (uint32_t)attn_lds(W::TILE, a.n_req), a);
     }
-    if constexpr (DT == RBT_DT_BF16) {
-        using Th = ThinShape<HDP>;
-        if (a.thin && e == hipSuccess)
-            e = ask_lds(attn_thin_kernel<HDP>, std::min(attn_lds(Th::TILE, kPagedMaxReq), kLdsBytes), asked_t);
-        if (a.thin && e == hipSuccess)
-            e = launch(L, attn_thin_kernel<HDP>, dim3(256 * Th::PER_CU), dim3(256), (uint32_t)attn_lds(Th::TILE, a.n_req), a);
+    if (a.thin && e == hipSuccess) {
+        e = ask_lds(attn_thin_kernel<DT, HDP>, std::min(attn_lds(Th::TILE, kPagedMaxReq), kLdsBytes), asked_t);
+        if (e == hipSuccess)
+            e = launch(L, attn_thin_kernel<DT, HDP>, dim3(256 * Th::PER_CU), dim3(256),
+                       (uint32_t)attn_lds(Th::TILE, a.n_req), a);
     }
     if (e != hipSuccess) return e;
     return launch(Lm, attn_merge_kernel<HDP>, dim3(1024), dim3(256), 0, a, (int)wide);
