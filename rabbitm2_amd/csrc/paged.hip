@@ -238,7 +238,8 @@ struct AttnArgs {
     PagedDims d;
     int n_req, max_blocks, T, n_heads, window;
     PageDiv group; // query heads to a key/value head
-    int thin;      // whether requests of up to 16 rows have a launch of their own
+    int thin;      // whether requests of up to 16 rows are the thin blocks'
+    int wide;      // whether there are wide blocks
     float scale2;  // scale * log2(e), into the query rows: the softmax runs in powers of two
     const int32_t *tables, *kv_len, *q_start;
     const void *kc, *vc;
@@ -354,7 +355,8 @@ __global__ __launch_bounds__(256) void attn_any_kernel(AttnArgs a) {
 // its positions in tiles, staged in LDS as bf16 parts:
 //   wide   128 rows, 32 to a wave; the block's waves share each tile of keys and values
 //   thin   requests of up to 16 rows (a decoding token): each wave takes tiles of 32 positions of its own
-// in two launches, and long ranges are cut into chunks that different blocks take, joined by a third.
+// each kind by blocks of its own, and long ranges are cut into pieces that different blocks take, joined by
+// attn_merge_kernel.
 //
 // Products: v_mfma_f32_16x16x32_bf16, transposed so that nothing moves between lanes: S^T = K Q^T leaves lane
 // (c = l % 16, g = l / 16) the scores of query c with keys 4 g + i of two 16-key groups, which as they stand are
@@ -465,11 +467,11 @@ struct ScheduleShared {
     int any[4], sum[4][3];
 };
 template <bool THIN, int HDP>
-__device__ int schedule(const AttnArgs &a, int32_t *s_items, int32_t *s_units, ScheduleShared &s) {
+__device__ int schedule(const AttnArgs &a, int block, int blocks, int32_t *s_items, int32_t *s_units, ScheduleShared &s) {
     constexpr int tr = kTileRows<THIN>, kUnits = AttnWs<THIN>::max_units(HDP);
     const int per = (a.n_req + 255) / 256, r0 = min(a.n_req, (int)threadIdx.x * per), r1 = min(a.n_req, r0 + per);
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-    AttnHeader *hdr = blockIdx.x == 0 ? AttnWs<THIN>::header(a.ws) : nullptr;  // one block tells the merge launch
+    AttnHeader *hdr = block == 0 ? AttnWs<THIN>::header(a.ws) : nullptr;  // one block tells the merge launch
     // the first request of a thread (all of them, up to 256 requests) stays in registers
     Request first{};
     if (r0 < r1) first = request(a, r0);
@@ -494,7 +496,7 @@ __device__ int schedule(const AttnArgs &a, int32_t *s_items, int32_t *s_units, S
         if (hdr && threadIdx.x == 0) hdr->merge_blocks = 0;
         return 0;
     }
-    work = ((s.work[0] + s.work[1]) + (s.work[2] + s.work[3])) * (float)a.d.n_kv / (float)(2 * gridDim.x);
+    work = ((s.work[0] + s.work[1]) + (s.work[2] + s.work[3])) * (float)a.d.n_kv / (float)(2 * blocks);
     int chunk = (int)fminf(work, 1.0e9f) / 128 * 128 + 128;
     for (;;) {
         int v[3] = {0, 0, 0}, inc[3], before[3], total[3];  // items, partial units, merge blocks
@@ -995,17 +997,17 @@ __device__ __forceinline__ Item item_of(const AttnArgs &a, int it, int chunk, co
 // L2. A block starts with the item of its own number and then takes the next one left of its eighth, then of the other
 // eighths: ask() early, its answer used by next() at the item's end.
 struct ItemQueue {
-    int it, n, xcd;  // it < 0: nothing is left
+    int it, n, xcd, per;  // it < 0: nothing is left
     AttnHeader *hdr;
     __device__ __forceinline__ int start(int x) const { return (int)((long long)n * x / 8); }
-    __device__ __forceinline__ ItemQueue(int n_items, AttnHeader *header) : n(n_items), xcd(blockIdx.x & 7), hdr(header) {
-        it = start(xcd) + (int)(blockIdx.x >> 3);
+    __device__ __forceinline__ ItemQueue(int n_items, AttnHeader *header, int block, int blocks)
+        : n(n_items), xcd(block & 7), per(blocks >> 3), hdr(header) {
+        it = start(xcd) + (block >> 3);
         if (it >= start(xcd + 1)) it = -1;
     }
     __device__ __forceinline__ int ask() const { return threadIdx.x == 0 ? atomicAdd(&hdr->taken[xcd][0], 1) : 0; }
     // for all threads
     __device__ __forceinline__ void next(int ticket, int *s_next) {
-        const int per = (int)(gridDim.x >> 3);
         for (;;) {
             if (threadIdx.x < kWave) {  // the answer, or the first other eighth with any left (its counters only grow)
                 const int x = threadIdx.x & 7;
@@ -1069,7 +1071,7 @@ __device__ __forceinline__ void again_rows(const AttnArgs &a, const Item &x, con
 }
 
 // LDS: [tile | row_any's][pages' places][item and unit prefix sums]
-constexpr int kLdsBytes = 159 << 10;  // of 160 KiB: the kernels' fixed shared variables take less than the last
+constexpr int kLdsBytes = 156 << 10;  // of 160 KiB: the kernels' fixed shared variables take less than the rest
 constexpr int attn_lds(int tile, int n_req) { return tile + kTabBytes + 8 * (n_req + 1); }
 
 // A thin wave on an f32 cache: v_mfma_f32_16x16x4_f32 on f32 operands straight from the cache, 16 positions at a time (a
@@ -1171,8 +1173,9 @@ struct ThinShape {
     static_assert(ROWS <= WAVE, "a wave's rows fit its tile");
     static_assert(sizeof(RowShared) <= (size_t)TILE, "row_any's LDS");
 };
+// Blocks `block` of `blocks`, a multiple of eight.
 template <int DT, int HDP>
-__global__ __launch_bounds__(256, (ThinShape<DT, HDP>::PER_CU)) void attn_thin_kernel(AttnArgs a) {
+__device__ __forceinline__ void attn_thin(const AttnArgs &a, int block, int blocks) {
     constexpr int WAVE = ThinShape<DT, HDP>::WAVE;
     __shared__ ScheduleShared s_sched;
     __shared__ float s_m[4][kThinRows], s_l[4][kThinRows];
@@ -1180,9 +1183,9 @@ __global__ __launch_bounds__(256, (ThinShape<DT, HDP>::PER_CU)) void attn_thin_k
     uint64_t *s_tab = reinterpret_cast<uint64_t *>(smem + ThinShape<DT, HDP>::TILE);
     int32_t *s_items = reinterpret_cast<int32_t *>(s_tab + kTabPages), *s_units = s_items + a.n_req + 1;
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
-    const int chunk = __builtin_amdgcn_readfirstlane(schedule<true, HDP>(a, s_items, s_units, s_sched));
+    const int chunk = __builtin_amdgcn_readfirstlane(schedule<true, HDP>(a, block, blocks, s_items, s_units, s_sched));
     if (chunk == 0) return;
-    ItemQueue items(__builtin_amdgcn_readfirstlane(s_items[a.n_req]), AttnWs<true>::header(a.ws));
+    ItemQueue items(__builtin_amdgcn_readfirstlane(s_items[a.n_req]), AttnWs<true>::header(a.ws), block, blocks);
     const int span = tab_span(a);
     const PaddedTile<HDP> tl;
     while (items.it >= 0) {
@@ -1319,16 +1322,16 @@ struct WideShape {
     static_assert(sizeof(RowShared) <= (size_t)TILE, "row_any's LDS");
 };
 template <int DT, int HDP>
-__global__ __launch_bounds__(256, (WideShape<DT, HDP>::PER_CU)) void attn_wide_kernel(AttnArgs a) {
+__device__ __forceinline__ void attn_wide(const AttnArgs &a, int block, int blocks) {
     using Sh = WideShape<DT, HDP>;
     __shared__ ScheduleShared s_sched;
     __shared__ int s_flag[kWideRows], s_next;
     uint64_t *s_tab = reinterpret_cast<uint64_t *>(smem + Sh::TILE);
     int32_t *s_items = reinterpret_cast<int32_t *>(s_tab + kTabPages), *s_units = s_items + a.n_req + 1;
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
-    const int chunk = __builtin_amdgcn_readfirstlane(schedule<false, HDP>(a, s_items, s_units, s_sched));
+    const int chunk = __builtin_amdgcn_readfirstlane(schedule<false, HDP>(a, block, blocks, s_items, s_units, s_sched));
     if (chunk == 0) return;
-    ItemQueue items(__builtin_amdgcn_readfirstlane(s_items[a.n_req]), AttnWs<false>::header(a.ws));
+    ItemQueue items(__builtin_amdgcn_readfirstlane(s_items[a.n_req]), AttnWs<false>::header(a.ws), block, blocks);
     const int span = tab_span(a);
     const typename Sh::Tile tl;
     while (items.it >= 0) {
@@ -1432,6 +1435,25 @@ __global__ __launch_bounds__(256, (WideShape<DT, HDP>::PER_CU)) void attn_wide_k
     }
 }
 
+// One launch of both: the wide launch's blocks first, which leave at once where no request is theirs; the thin ones
+// fill the places that the last wide ones leave (in launches of their own: prompts and decoding rows mixed 33.6 against
+// @MIX@ us, 32 decoding sequences @DEC@).
+template <int DT, int HDP>
+struct AttnShape {
+    static constexpr int TILE = std::max(WideShape<DT, HDP>::TILE, ThinShape<DT, HDP>::TILE);
+    static constexpr int PER_CU = WideShape<DT, HDP>::PER_CU, BLOCKS = 256 * PER_CU;
+    static_assert(PER_CU == ThinShape<DT, HDP>::PER_CU, "one launch bound");
+};
+template <int DT, int HDP>
+__global__ __launch_bounds__(256, (AttnShape<DT, HDP>::PER_CU)) void attn_kernel(AttnArgs a) {
+    constexpr int n = AttnShape<DT, HDP>::BLOCKS;
+    const int b = (int)blockIdx.x;
+    if (b < a.wide * n)
+        attn_wide<DT, HDP>(a, b, n);
+    else
+        attn_thin<DT, HDP>(a, b - a.wide * n, n);
+}
+
 // The pieces of cut tiles joined: out = sum_i w_i o_i / sum_i w_i l_i with w_i = 2^(m_i - max m), HDP / 4 lanes to a row.
 template <int HDP, bool THIN>
 __device__ __forceinline__ void merge_block(const AttnArgs &a, const AttnHeader *hdr, int id, float (*s_state)[4][2],
@@ -1505,14 +1527,13 @@ __device__ __forceinline__ void merge_block(const AttnArgs &a, const AttnHeader 
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
     *reinterpret_cast<f32x4 *>(a.out + (size_t)pl.t * a.out_stride + (size_t)pl.h * a.d.hd + 4 * sub) = o * inv;
 }
-// wide: whether the wide launch ran before.
 template <int HDP>
-__global__ __launch_bounds__(256) void attn_merge_kernel(AttnArgs a, int wide) {
+__global__ __launch_bounds__(256) void attn_merge_kernel(AttnArgs a) {
     __shared__ float s_state[4][4][2];
     __shared__ f32x4 s_o[4][64];
     AttnHeader *hw = AttnWs<false>::header(a.ws), *ht = AttnWs<true>::header(a.ws);
     if (blockIdx.x == 0 && threadIdx.x < 8) hw->taken[threadIdx.x][0] = ht->taken[threadIdx.x][0] = 0;
-    const int nw = wide ? hw->merge_blocks : 0, nt = a.thin ? ht->merge_blocks : 0;
+    const int nw = a.wide ? hw->merge_blocks : 0, nt = a.thin ? ht->merge_blocks : 0;
     for (int id = blockIdx.x; id < nw + nt; id += gridDim.x)
         if (id < nt)
             merge_block<HDP, true>(a, ht, id, s_state, s_o);
@@ -1604,31 +1625,21 @@ hipError_t ask_lds(F kernel, int bytes, std::atomic<uint64_t> &asked) {
 
 template <int DT, int HDP>
 hipError_t launch_attn(const Launch &L, const Launch &Lm, AttnArgs a) {
-    using W = WideShape<DT, HDP>;
+    using Sh = AttnShape<DT, HDP>;
     const int G = a.n_heads / a.d.n_kv;
-    // Requests of up to 16 rows have a launch of their own, where its tiles and the step's prefix sums fit LDS (a bf16
-    // cache with head dims above 128: up to 2900 requests). A launch that no request can belong to is left out;
-    // otherwise each finds its requests on the device.
-    using Th = ThinShape<DT, HDP>;
-    a.thin = G <= kThinRows && attn_lds(Th::TILE, a.n_req) <= kLdsBytes;
-    const bool wide = !a.thin || (int64_t)a.T * G > kThinRows;
-    static std::atomic<uint64_t> asked_w{0}, asked_t{0};
-    hipError_t e = hipSuccess;
-    if (wide) {
-        static_assert(attn_lds(W::TILE, kPagedMaxReq) <= kLdsBytes, "the wide launch takes any step");
-        e = ask_lds(attn_wide_kernel<DT, HDP>, attn_lds(W::TILE, kPagedMaxReq), asked_w);
-        if (e == hipSuccess)
-            e = launch(a.thin ? Lm : L, attn_wide_kernel<DT, HDP>, dim3(256 * W::PER_CU), dim3(256),
-                       (uint32_t)attn_lds(W::TILE, a.n_req), a);
-    }
-    if (a.thin && e == hipSuccess) {
-        e = ask_lds(attn_thin_kernel<DT, HDP>, std::min(attn_lds(Th::TILE, kPagedMaxReq), kLdsBytes), asked_t);
-        if (e == hipSuccess)
-            e = launch(L, attn_thin_kernel<DT, HDP>, dim3(256 * Th::PER_CU), dim3(256),
-                       (uint32_t)attn_lds(Th::TILE, a.n_req), a);
-    }
+    // Requests of up to 16 rows have blocks of their own, where their tiles and the step's prefix sums fit LDS (a bf16
+    // cache with head dims above 128: up to 2500 requests). Blocks that no request can belong to are left out;
+    // otherwise each kind finds its requests on the device.
+    a.thin = G <= kThinRows && attn_lds(Sh::TILE, a.n_req) <= kLdsBytes;
+    a.wide = !a.thin || (int64_t)a.T * G > kThinRows;
+    const int lds = attn_lds(a.thin ? Sh::TILE : WideShape<DT, HDP>::TILE, a.n_req);
+    static_assert(attn_lds(WideShape<DT, HDP>::TILE, kPagedMaxReq) <= kLdsBytes, "wide blocks take any step");
+    static std::atomic<uint64_t> asked{0};
+    hipError_t e = ask_lds(attn_kernel<DT, HDP>, kLdsBytes, asked);
+    if (e == hipSuccess)
+        e = launch(L, attn_kernel<DT, HDP>, dim3((unsigned)(Sh::BLOCKS * (a.wide + a.thin))), dim3(256), (uint32_t)lds, a);
     if (e != hipSuccess) return e;
-    return launch(Lm, attn_merge_kernel<HDP>, dim3(1024), dim3(256), 0, a, (int)wide);
+    return launch(Lm, attn_merge_kernel<HDP>, dim3(1024), dim3(256), 0, a);
 }
 }  // namespace
 
