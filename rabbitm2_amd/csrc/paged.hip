@@ -16,12 +16,24 @@ namespace {
 
 typedef __bf16 bf16_t;
 
+// Inclusive prefix sum over the wave, by DPP: within rows of 16 lanes, then the rows' totals handed on.
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr:1
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
+    return v;
+}
+
 // ---------------------------------------------------------------- plan
-// One block: three prefix sums over the requests (new rows, blocks needed, blocks given back) in LDS, then the
-// blocks pushed and popped and the rows' slots, each by its place in those sums (a binary search), so that one
-// long request costs no more than many short ones. All of it is latency; the sums are 64-bit, so that no input
-// can wrap them.
-constexpr int kPlanThreads = 1024, kPlanPer = kPagedMaxReq / kPlanThreads;
+// One block: three prefix sums over the requests (new rows, blocks needed, blocks given back), then the blocks pushed
+// and popped and the rows' slots, each by its place in those sums (a binary search in LDS), so that one long request
+// costs no more than many short ones. All of it is latency, so a new row's block is taken from the free stack, not from
+// the table entry that another thread is writing. Steps of many rows give those to a launch of their own (1024 requests,
+// 32768 rows: @PLAN@).
+constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / kWave, kPlanPer = kPagedMaxReq / kPlanThreads;
 
 struct PlanArgs {
     int n_req, max_blocks, n_blocks, max_tokens;
@@ -30,122 +42,112 @@ struct PlanArgs {
     int32_t *tables, *free_list, *kv_len, *n_free_out, *q_start, *slots, *positions, *status;
 };
 
-// The block's exclusive prefix sums of three values per thread; tot: the sums of all.
-__device__ __forceinline__ void block_scan3(long long (&v)[3], long long (&tot)[3], long long (*s_w)[3]) {
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-    long long inc[3];
-#pragma unroll
-    for (int i = 0; i < 3; ++i) inc[i] = v[i];
-    for (int off = 1; off < kWave; off <<= 1)
-#pragma unroll
-        for (int i = 0; i < 3; ++i) {
-            const long long up = __shfl_up(inc[i], off, kWave);
-            if (lane >= off) inc[i] += up;
-        }
-    if (lane == kWave - 1)
-#pragma unroll
-        for (int i = 0; i < 3; ++i) s_w[wv][i] = inc[i];
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-        long long before = 0;
-        tot[i] = 0;
-        for (int w = 0; w < kPlanThreads / kWave; ++w) {
-            if (w < wv) before += s_w[w][i];
-            tot[i] += s_w[w][i];
-        }
-        v[i] = before + inc[i] - v[i];
-    }
+__device__ __forceinline__ int pages_for(int n, const PageDiv &div) {
+    const int p = (int)page_of((uint32_t)n, div);
+    return p + (n - p * (int)div.d > 0);
 }
-
-// The slot and position of row t of a step whose requests start at `start`.
-__device__ __forceinline__ void plan_row(const PlanArgs &a, const int32_t *start, int t, int r, int base) {
-    const int pos = base + (t - start[r]), page = (int)page_of((uint32_t)pos, a.div);
-    const int b = a.tables[(size_t)r * a.max_blocks + page];
-    const bool in = b >= 0 && b < a.n_blocks;
-    a.slots[t] = in ? b * (int)a.div.d + (pos - page * (int)a.div.d) : -1;
+__device__ __forceinline__ void plan_put(const PlanArgs &a, int t, int pos, int page, int b) {
+    a.slots[t] = b >= 0 && b < a.n_blocks ? b * (int)a.div.d + (pos - page * (int)a.div.d) : -1;
     a.positions[t] = pos;
 }
 
 // rows: whether this launch fills slots and positions too (else plan_rows_kernel does).
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a, int rows) {
     __shared__ int32_t s_start[kPagedMaxReq + 1], s_need[kPagedMaxReq], s_freed[kPagedMaxReq], s_len[kPagedMaxReq];
-    __shared__ long long s_w[kPlanThreads / kWave][3];
+    __shared__ int s_sum[kPlanWaves][3];
+    __shared__ float s_big[kPlanWaves];
     __shared__ int s_bad;
-    const int tid = threadIdx.x, bs = (int)a.div.d;
-    const long long room = (long long)a.max_blocks * bs;
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, bs = (int)a.div.d;
     const int count = a.n_free[0];
+    const int per = (a.n_req + kPlanThreads - 1) / kPlanThreads;  // requests tid * per + i
+    int len[kPlanPer], add[kPlanPer], need[kPlanPer], freed[kPlanPer];
     if (tid == 0) s_bad = count < 0 || count > a.n_blocks;
-    int len[kPlanPer], add[kPlanPer], need[kPlanPer], have[kPlanPer];  // requests tid * kPlanPer + i
-    bool bad = false, ends[kPlanPer];
-    long long v[3] = {0, 0, 0}, tot[3];
+    bool bad = false;
+    float big = 0.0f;
+    int v[3] = {0, 0, 0}, inc[3], before[3], total[3];
 #pragma unroll
     for (int i = 0; i < kPlanPer; ++i) {
-        const int r = tid * kPlanPer + i;
-        const bool live = r < a.n_req;
-        len[i] = live ? a.len[r] : 0;
-        const int nl = live ? a.new_len[r] : 0;
-        ends[i] = nl < 0;
+        const int r = tid * per + i;
+        len[i] = add[i] = need[i] = freed[i] = 0;
+        if (i >= per || r >= a.n_req) continue;
+        const int n = a.len[r], nl = a.new_len[r];
+        len[i] = n;
         add[i] = max(nl, 0);
-        const bool out = len[i] < 0 || (long long)len[i] + add[i] > room;
+        const bool out = n < 0 || (long long)n + add[i] > (long long)a.max_blocks * bs;
         bad |= out;
-        const int n0 = out ? 0 : len[i], n1 = out ? 0 : len[i] + add[i];
-        have[i] = (int)page_of((uint32_t)n0, a.div) + (n0 % bs != 0);
-        need[i] = ends[i] ? 0 : (int)page_of((uint32_t)n1, a.div) + (n1 % bs != 0) - have[i];
+        const int have = out ? 0 : pages_for(n, a.div);
+        need[i] = out || nl < 0 ? 0 : pages_for(n + add[i], a.div) - have;
+        freed[i] = nl < 0 ? have : 0;
         v[0] += add[i];
         v[1] += need[i];
-        v[2] += ends[i] ? have[i] : 0;
+        v[2] += freed[i];
+        big += (float)add[i] + (float)need[i] + (float)freed[i];
     }
+    // the 32-bit sums hold where their sum in floats, no part of which is negative, is below 2^30
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        inc[i] = wave_scan(v[i]);
+        if (lane == kWave - 1) s_sum[wv][i] = inc[i];
+    }
+    big = wave_sum(big);
+    if (lane == 0) s_big[wv] = big;
     __syncthreads();
     if (bad) s_bad = 1;
-    block_scan3(v, tot, s_w);
-    __syncthreads();
-    const long long top = count + tot[2];
-    const bool invalid = s_bad || tot[0] > a.max_tokens || top > a.n_blocks;
-    const long long lack = invalid ? 0 : tot[1] - top;
-    const bool ok = !invalid && lack <= 0;
-    if (tid == 0) {
-        a.status[0] = invalid ? -1 : lack > 0 ? (int)lack : 0;
-        a.n_free_out[0] = ok ? (int)(top - tot[1]) : count;
-        a.q_start[a.n_req] = s_start[a.n_req] = ok ? (int)tot[0] : 0;
+    big = 0.0f;
+    for (int w = 0; w < kPlanWaves; ++w) big += s_big[w];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {  // the waves before this one, and all
+        const int x = wave_scan(lane < kPlanWaves ? s_sum[lane][i] : 0);
+        total[i] = __builtin_amdgcn_readlane(x, kPlanWaves - 1);
+        before[i] = inc[i] - v[i] + (wv > 0 ? __builtin_amdgcn_readlane(x, max(wv - 1, 0)) : 0);
     }
-    const int n_need = ok ? (int)tot[1] : 0, n_freed = ok ? (int)tot[2] : 0;
+    __syncthreads();
+    const bool valid = !s_bad && big < 1073741824.0f && total[0] <= a.max_tokens && count + total[2] <= a.n_blocks;
+    const int top = count + total[2], lack = valid ? max(total[1] - top, 0) : 0;
+    const bool ok = valid && lack == 0;
+    if (tid == 0) {
+        a.status[0] = valid ? lack : -1;
+        a.n_free_out[0] = ok ? top - total[1] : count;
+        a.q_start[a.n_req] = s_start[a.n_req] = ok ? total[0] : 0;
+    }
 #pragma unroll
     for (int i = 0; i < kPlanPer; ++i) {
-        const int r = tid * kPlanPer + i;
-        if (r < a.n_req) {
-            s_start[r] = ok ? (int)v[0] : 0;
-            s_need[r] = ok ? (int)v[1] : 0;
-            s_freed[r] = ok ? (int)v[2] : 0;
-            s_len[r] = len[i];
-            a.q_start[r] = s_start[r];
-            a.kv_len[r] = !ok ? len[i] : ends[i] ? 0 : len[i] + add[i];
+        const int r = tid * per + i;
+        if (i >= per || r >= a.n_req) continue;
+        s_start[r] = ok ? before[0] : 0;
+        s_need[r] = ok ? before[1] : 0;
+        s_freed[r] = ok ? before[2] : 0;
+        s_len[r] = len[i];
+        a.q_start[r] = s_start[r];
+        a.kv_len[r] = !ok ? len[i] : a.new_len[r] < 0 ? 0 : len[i] + add[i];
+        before[0] += add[i];
+        before[1] += need[i];
+        before[2] += freed[i];
+    }
+    __syncthreads();
+    if (ok && total[2] > 0) {
+        for (int i = tid; i < total[2]; i += kPlanThreads) {
+            const int r = request_of(s_freed, a.n_req, i);
+            a.free_list[count + i] = a.tables[(size_t)r * a.max_blocks + (i - s_freed[r])];
         }
-        v[0] += add[i];
-        v[1] += need[i];
-        v[2] += ends[i] ? have[i] : 0;
+        __syncthreads();  // they may be popped again
     }
-    __syncthreads();
-    for (int i = tid; i < n_freed; i += kPlanThreads) {
-        const int r = request_of(s_freed, a.n_req, i);
-        a.free_list[count + i] = a.tables[(size_t)r * a.max_blocks + (i - s_freed[r])];
-    }
-    __syncthreads();
-    for (int i = tid; i < n_need; i += kPlanThreads) {
-        const int r = request_of(s_need, a.n_req, i), n0 = s_len[r];
-        const int first = (int)page_of((uint32_t)n0, a.div) + (n0 % bs != 0);
-        a.tables[(size_t)r * a.max_blocks + first + (i - s_need[r])] = a.free_list[(int)top - 1 - i];
-    }
+    if (ok)
+        for (int i = tid; i < total[1]; i += kPlanThreads) {
+            const int r = request_of(s_need, a.n_req, i);
+            a.tables[(size_t)r * a.max_blocks + pages_for(s_len[r], a.div) + (i - s_need[r])] = a.free_list[top - 1 - i];
+        }
     if (!rows) return;
-    __syncthreads();
     const int T = s_start[a.n_req];
     for (int t = tid; t < a.max_tokens; t += kPlanThreads) {
-        if (t < T) {
-            const int r = request_of(s_start, a.n_req, t);
-            plan_row(a, s_start, t, r, s_len[r]);
-        } else {
+        if (t >= T) {
             a.slots[t] = a.positions[t] = -1;
+            continue;
         }
+        const int r = request_of(s_start, a.n_req, t), pos = s_len[r] + (t - s_start[r]);
+        const int page = (int)page_of((uint32_t)pos, a.div), have = pages_for(s_len[r], a.div);
+        plan_put(a, t, pos, page,
+                 page < have ? a.tables[(size_t)r * a.max_blocks + page] : a.free_list[top - 1 - (s_need[r] + page - have)]);
     }
 }
 
@@ -156,8 +158,9 @@ __global__ __launch_bounds__(256) void plan_rows_kernel(PlanArgs a) {
         a.slots[t] = a.positions[t] = -1;
         return;
     }
-    const int r = request_of(a.q_start, a.n_req, t);
-    plan_row(a, a.q_start, t, r, a.kv_len[r] - (a.q_start[r + 1] - a.q_start[r]));
+    const int r = request_of(a.q_start, a.n_req, t), pos = a.kv_len[r] - a.q_start[r + 1] + t;
+    const int page = (int)page_of((uint32_t)pos, a.div);
+    plan_put(a, t, pos, page, a.tables[(size_t)r * a.max_blocks + page]);
 }
 
 // ---------------------------------------------------------------- append
@@ -231,6 +234,126 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     auto at = [&](int i) { return paged_row(a.d, b, i / hd, off) + (uint64_t)(i % hd); };
     rows(k, a.k_norm, inv_k, kvd, [&](int i, float x) { store_kv<DT>(a.kc, at(i), x); });
     for (int i = tid; i < kvd; i += 256) store_kv<DT>(a.vc, at(i), v[i]);
+}
+
+// The same for head dims that are multiples of 8 and 16-byte aligned rows of up to 256 * 8 * kAppendQ floats of q and
+// 256 * 8 * kAppendK of k: everything is asked for at once (the rows whether or not the token has a slot), held in
+// registers through the norm, and each thread turns whole quads of pairs (elements 4 i .. 4 i + 3 of a head's halves).
+constexpr int kAppendQ = 4, kAppendK = 2;
+__device__ __forceinline__ void store4(float *p, f32x4 v) { *reinterpret_cast<f32x4 *>(p) = v; }
+template <int DT>
+__device__ __forceinline__ void store_kv4(void *p, uint64_t i, f32x4 v) {
+    if constexpr (DT == RBT_DT_F32) {
+        store4(static_cast<float *>(p) + i, v);
+    } else {
+        typedef bf16_t bf16x4 __attribute__((ext_vector_type(4)));
+        *reinterpret_cast<bf16x4 *>(static_cast<bf16_t *>(p) + i) = __builtin_convertvector(v, bf16x4);
+    }
+}
+template <int N>
+struct AppendRow {
+    f32x4 lo[N], hi[N], wl[N], wh[N], c0[N], c1[N];  // halves, their norm weights, (cos, sin) of the four pairs
+    __device__ __forceinline__ void load(const float *src, const float *w, int quads, int per_half, int hd) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int u = min((int)threadIdx.x + 256 * i, quads - 1), h = u / per_half, at = h * hd + 4 * (u - h * per_half);
+            lo[i] = ld_f4(src + at);
+            hi[i] = ld_f4(src + at + hd / 2);
+            if (w) {
+                wl[i] = ld_f4(w + at);
+                wh[i] = ld_f4(w + at + hd / 2);
+            }
+        }
+    }
+    __device__ __forceinline__ void load_turns(const float *cs, int quads, int per_half) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int u = min((int)threadIdx.x + 256 * i, quads - 1), q = u % per_half;
+            c0[i] = ld_f4(cs + 8 * q);
+            c1[i] = ld_f4(cs + 8 * q + 4);
+        }
+    }
+    __device__ __forceinline__ float squares(int quads) const {
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if ((int)threadIdx.x + 256 * i < quads)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s += lo[i][j] * lo[i][j] + hi[i][j] * hi[i][j];
+        return s;
+    }
+    // put(element, four values) of both halves, normed and turned
+    template <typename Put>
+    __device__ __forceinline__ void finish(bool norm, float inv, bool turn, int quads, int per_half, int hd, Put put) {
+#pragma clang fp contract(off)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int u = (int)threadIdx.x + 256 * i;
+            if (u >= quads) break;
+            const int h = u / per_half, at = h * hd + 4 * (u - h * per_half);
+            f32x4 x = lo[i], y = hi[i];
+            if (norm) {
+                x = x * inv * wl[i];
+                y = y * inv * wh[i];
+            }
+            if (turn) {
+                const f32x4 c = f32x4{c0[i].x, c0[i].z, c1[i].x, c1[i].z}, s = f32x4{c0[i].y, c0[i].w, c1[i].y, c1[i].w};
+                const f32x4 a = x * c - y * s, b = y * c + x * s;
+                x = a;
+                y = b;
+            }
+            put(at, x);
+            put(at + hd / 2, y);
+        }
+    }
+};
+template <int DT>
+__global__ __launch_bounds__(256) void append_quads_kernel(AppendArgs a) {
+    __shared__ float red[8];
+    const int t = blockIdx.x, lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    const int hd = a.d.hd, per_half = hd / 8, qd = a.n_heads * hd, kvd = a.d.n_kv * hd, q_quads = a.q ? qd / 8 : 0;
+    const int slot = a.slots[t], pos = a.rope ? a.positions[t] : 0;
+    AppendRow<kAppendQ> q;
+    AppendRow<kAppendK> k;
+    f32x4 v[2 * kAppendK];
+    if (a.q) q.load(a.q + (size_t)t * a.q_stride, a.q_norm, q_quads, per_half, hd);
+    k.load(a.k + (size_t)t * a.k_stride, a.k_norm, kvd / 8, per_half, hd);
+#pragma unroll
+    for (int i = 0; i < 2 * kAppendK; ++i)
+        v[i] = ld_f4(a.v + (size_t)t * a.v_stride + 4 * min((int)threadIdx.x + 256 * i, kvd / 4 - 1));
+    if (slot < 0 || slot >= a.d.n_blocks * a.d.block_size || (a.rope && (pos < 0 || pos >= a.n_rope))) return;
+    if (a.rope) {
+        const float *cs = reinterpret_cast<const float *>(a.rope + (size_t)pos * (hd / 2));
+        if (a.q) q.load_turns(cs, q_quads, per_half);
+        k.load_turns(cs, kvd / 8, per_half);
+    }
+    float inv_q = 1.0f, inv_k = 1.0f;
+    if (a.q_norm || a.k_norm) {  // the same for all threads
+        float sq = a.q && a.q_norm ? q.squares(q_quads) : 0.0f, sk = a.k_norm ? k.squares(kvd / 8) : 0.0f;
+        sq = wave_sum(sq);
+        sk = wave_sum(sk);
+        if (lane == 0) {
+            red[wv] = sq;
+            red[4 + wv] = sk;
+        }
+        __syncthreads();
+        sq = (red[0] + red[1]) + (red[2] + red[3]);
+        sk = (red[4] + red[5]) + (red[6] + red[7]);
+        inv_q = 1.0f / sqrtf(sq / (float)qd + a.eps);
+        inv_k = 1.0f / sqrtf(sk / (float)kvd + a.eps);
+    }
+    const int b = (int)page_of((uint32_t)slot, a.d.div), off = slot - b * a.d.block_size;
+    const bool turn = a.rope != nullptr;
+    if (a.q)
+        q.finish(a.q_norm != nullptr, inv_q, turn, q_quads, per_half, hd,
+                 [&](int i, f32x4 x) { store4(a.q_out + (size_t)t * qd + i, x); });
+    auto at = [&](int i) { return paged_row(a.d, b, i / hd, off) + (uint64_t)(i % hd); };
+    k.finish(a.k_norm != nullptr, inv_k, turn, kvd / 8, per_half, hd, [&](int i, f32x4 x) { store_kv4<DT>(a.kc, at(i), x); });
+#pragma unroll
+    for (int i = 0; i < 2 * kAppendK; ++i) {
+        const int u = (int)threadIdx.x + 256 * i;
+        if (u < kvd / 4) store_kv4<DT>(a.vc, at(4 * u), v[i]);
+    }
 }
 
 // ---------------------------------------------------------------- attention
@@ -446,17 +569,6 @@ __device__ __forceinline__ Pieces pieces_of(const Cut &c, int t) {
 constexpr int kMergeManyPieces = 16;
 template <int HDP>
 __device__ __forceinline__ int merge_rows(int nc) { return 256 / HDP * (nc >= kMergeManyPieces ? 1 : 4); }
-
-// Inclusive prefix sum over the wave, by DPP: within rows of 16 lanes, then the rows' totals handed on.
-__device__ __forceinline__ int wave_scan(int v) {
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr:1
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
-    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
-    return v;
-}
 
 // A launch's items (request, head, row tile, piece), by every block for itself: prefix sums over the requests into
 // s_items [n_req + 1] and s_units. The chunk length spreads the work over about two rounds of blocks; it doubles
@@ -1604,6 +1716,12 @@ hipError_t launch_paged_append(const Launch &L, const rbt_paged_kv &kv, const rb
     a.kc = kv.k;
     a.vc = kv.v;
     const dim3 g((unsigned)w.n_tokens);
+    const auto a16 = [](const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
+    if (kv.head_dim % 8 == 0 && qd <= 2048 * kAppendQ && kvd <= 2048 * kAppendK && a16(w.q) && a16(w.k) && a16(w.v) &&
+        a16(w.q_out) && a16(w.q_norm) && a16(w.k_norm) && a16(w.rope) && a16(kv.k) && a16(kv.v) && a.q_stride % 4 == 0 &&
+        a.k_stride % 4 == 0 && a.v_stride % 4 == 0 && a.d.block_stride % 4 == 0)
+        return kv.dtype == RBT_DT_BF16 ? launch(L, append_quads_kernel<RBT_DT_BF16>, g, dim3(256), 0, a)
+                                       : launch(L, append_quads_kernel<RBT_DT_F32>, g, dim3(256), 0, a);
     return kv.dtype == RBT_DT_BF16 ? launch(L, append_kernel<RBT_DT_BF16>, g, dim3(256), 0, a)
                                    : launch(L, append_kernel<RBT_DT_F32>, g, dim3(256), 0, a);
 }
