@@ -882,35 +882,43 @@ __device__ __forceinline__ void wave_init(WaveState<HDP, NQ, QP> &w, const AttnA
                                           int row0, int q_off) {
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, G = (int)a.group.d;
     w.q_at = q_off + c * PaddedTile<HDP>::ROW + 16 * g;
+    // Every load before the first answer is used. Past the head's end: its last 8 elements, as 0 (without a branch, which
+    // would make each load wait for the one before).
+    f32x4 x[NQ][HDP / 32][2];
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
         const int row = min(row0 + 16 * n + c, rows - 1), tok = (int)page_of((uint32_t)row, a.group);
         const float *src = a.q + (size_t)(q.t0 + tok) * a.q_stride + (size_t)(kvh * G + row - tok * G) * a.d.hd;
         w.pos[n] = q.p0 + tok;
+#pragma unroll
+        for (int st = 0; st < HDP / 32; ++st)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) x[n][st][i] = ld_f4(src + min(32 * st + 8 * g, a.d.hd - 8) + 4 * i);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
         w.m[n] = -INFINITY;
         w.l[n] = 0.0f;
 #pragma unroll
         for (int st = 0; st < HDP / 32; ++st) {
-            float x[8];
-            // past the head's end: its last 8 elements, as 0 (a branch here would make each load wait for the one before)
-            const int at = min(32 * st + 8 * g, a.d.hd - 8);
-            const f32x4 x0 = ld_f4(src + at), x1 = ld_f4(src + at + 4);
-            const float scale = at == 32 * st + 8 * g ? a.scale2 : 0.0f;
+            const float scale = 32 * st + 8 * g < a.d.hd ? a.scale2 : 0.0f;
+            float y[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                x[i] = x0[i] * scale;
-                x[4 + i] = x1[i] * scale;
-            }
+            for (int i = 0; i < 8; ++i) y[i] = x[n][st][i / 4][i % 4] * scale;
             u32x4 part[3];
-            split3(x, part, w.pc);
+            split3(y, part, w.pc);
 #pragma unroll
             for (int p = 0; p < QP; ++p) w.q[n][st][p] = part[p];
             if (QP < 3)
                 *reinterpret_cast<u32x4 *>(smem + w.q_at + n * 16 * PaddedTile<HDP>::ROW + st * 64) = part[2];
         }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
 #pragma unroll
         for (int d = 0; d < HDP / 16; ++d) w.o[n][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
 }
 
 // The places (byte offset of the block) of the pages that positions j0 .. j1 - 1 (at most tab_span of them, at least
