@@ -281,7 +281,9 @@ int rbt_hip_tensor(rbt_hip *h, const char *name, int layer, uint64_t *offset, ui
  * context): requests of any lengths share one pool of blocks ("pages") of block_size positions each. A step
  * runs rbt_hip_paged_plan_dev once, then per layer rbt_hip_paged_append_dev and rbt_hip_paged_attn_dev. All
  * take device pointers, are asynchronous on the handle stream and can be captured into a graph (after
- * rbt_hip_paged_reserve): every length is read on the device, so a captured step replays for other lengths. ---- */
+ * rbt_hip_paged_reserve): every length is read on the device, so a captured step replays for other lengths. The
+ * handle has one workspace, so its attention calls and the graphs that hold any run one after the other, as they
+ * do on its stream; a second handle has its own, and may share a cache. ---- */
 
 /* One layer's cache: block b's keys are k + b * block_stride, [n_kv_heads][block_size][head_dim] elements of
  * dtype (RBT_DT_F32 or RBT_DT_BF16), its values v + b * block_stride alike. block_stride 0: blocks follow each
@@ -356,10 +358,12 @@ int rbt_hip_paged_append_dev(rbt_hip *h, const rbt_paged_kv *kv, const rbt_paged
  * out[t][h] = sum_j softmax_j(scale * q[t][h] . k_j) v_j over the positions j of the request up to the row's own
  * p, with window > 0 over p - window + 1 .. p only. Query head h reads key/value head h / (n_heads /
  * n_kv_heads). q and out hold T rows of n_heads * head_dim floats, q_stride / out_stride floats apart (0: they
- * follow each other); scale 0: 1 / sqrt(head_dim). Sums and the softmax run in f32; the q rows enter the
- * products exactly, the weights with at least 16 bits. A position outside the table's length or on a block
- * outside [0, n_blocks) is not seen; a row that sees none is 0; rows of no request (behind the last one's)
- * are left as they are. What lies behind a row's own position, infinities and NaN too, does not reach it. */
+ * follow each other); out may be q where their strides agree, else they do not overlap. scale 0:
+ * 1 / sqrt(head_dim). Sums, the softmax and its weights are f32, keys and values enter the products exactly, the q
+ * rows times scale, rounded once in f32. A position outside the table's length or on a block outside [0, n_blocks) is
+ * not seen; a row that sees none is 0; rows of no request (behind the last one's) are left as they are. What lies
+ * behind a row's own position, infinities and NaN too, does not reach it. Head dims that are multiples of 8, with
+ * 16-byte aligned pointers, strides of a multiple of 16 bytes and blocks below 4 GiB, run on the matrix cores; any others run too, slowly. */
 int rbt_hip_paged_attn_dev(rbt_hip *h, const rbt_paged_kv *kv, const rbt_paged_batch *batch, const float *q,
                            uint64_t q_stride, int T, int n_heads, float scale, int window, float *out,
                            uint64_t out_stride);
@@ -384,8 +388,9 @@ void *rbt_hip_stream(rbt_hip *h); /* the hipStream_t all of this handle's work r
  * lists -- and "combine", and its "down_combine" is the down GEMM alone); rbt_hip_forward adds
  * "embed", "attn_norm", "qkv" (RMSNorm + q/k/v), "attention", "attn_merge", "wo", "ffn_norm",
  * "lm_head" (final norm + lm_head, with the argmax inside where the rows allow) and "argmax"
- * (otherwise); the paged cache's calls "paged_plan", "paged_append", "paged_attn" and "paged_merge". Batched steps launch fewer: from 512 (sequence, head) pairs the attention writes its
- * output without "attn_merge", and on the grouped path "combine" also runs the RMSNorm that the
+ * (otherwise); the paged cache's calls "paged_plan" ("paged_rows" too for steps of more than 2048 rows),
+ * "paged_append", "paged_attn" and, where the attention runs on the matrix cores, "paged_merge".
+ * Batched steps launch fewer: from 512 (sequence, head) pairs the attention writes its output without "attn_merge", and on the grouped path "combine" also runs the RMSNorm that the
  * next step would time as "attn_norm". rbt_hip_generate is never timed this way. Modes (on):
  *   0  off.
  *   1  each call waits for its own kernels and adds their durations (eager calls only).

@@ -52,12 +52,12 @@ enum ProfKernel {
     kProfRouter, kProfTopk, kProfGateup, kProfDown, kProfDispatch, kProfCombine,
     // the rest of the forward pass (rbt_hip_forward with profiling on)
     kProfEmbed, kProfAttnNorm, kProfQkv, kProfAttn, kProfAttnMerge, kProfWo, kProfFfnNorm, kProfLmHead, kProfArgmax,
-    kProfPagedPlan, kProfPagedAppend, kProfPagedAttn, kProfPagedMerge,
+    kProfPagedPlan, kProfPagedRows, kProfPagedAppend, kProfPagedAttn, kProfPagedMerge,
     kProfCount
 };
 const char *const kProfNames[kProfCount] = {"router", "topk", "gateup", "down_combine", "dispatch", "combine",
                                             "embed", "attn_norm", "qkv", "attention", "attn_merge", "wo", "ffn_norm",
-                                            "lm_head", "argmax", "paged_plan", "paged_append", "paged_attn",
+                                            "lm_head", "argmax", "paged_plan", "paged_rows", "paged_append", "paged_attn",
                                             "paged_merge"};
 
 // mode 1: one event pair per kernel kind, read after every call (each call waits for its work).
@@ -166,6 +166,7 @@ struct rbt_hip {
     // this device's scratch array (rbt_hip_moe_dev_noalloc), from hipGetSymbolAddress at init
     void *scratch = nullptr;
     void *paged_ws = nullptr;  // the paged attention's workspace (rbt_hip_paged_reserve)
+    bool paged_ws_stale = false;  // an attention launch left it without its merge
     // tiled copies of layers' experts for the 128-row grouped GEMMs (rbt_hip_prefill_layout), keyed by
     // the layer's expert blobs; built only when the caller asks, used while option "prefill_layout" is on
     std::vector<TiledLayer> tiled;
@@ -1698,6 +1699,8 @@ int check_paged_attn(rbt_hip *h, const rbt_paged_kv *kv, const rbt_paged_batch *
     const uint64_t qd = (uint64_t)n_heads * (uint64_t)kv->head_dim;
     if (!check_paged_stride(h, "paged_attn", "q", q_stride, qd) || !check_paged_stride(h, "paged_attn", "out", out_stride, qd))
         return 0;
+    if (out == q && out && (q_stride ? q_stride : qd) != (out_stride ? out_stride : qd))
+        return fail(h, "paged_attn: out is q, with another stride");
     if (!isfinite(scale)) return fail(h, "paged_attn: scale is not finite");
     if (window < 0) return fail(h, "paged_attn: negative window");
     if (b->n_req > 0 && T > 0 && (!b->tables || !b->kv_len || !b->q_start || !q || !out))
@@ -1714,7 +1717,7 @@ int paged_ws_reserve(rbt_hip *h) {
         return fail(h, "paged_attn: the stream is being captured before rbt_hip_paged_reserve");
     void *ws = nullptr;
     HIP_OK(h, hipMalloc(&ws, kPagedWsBytes));
-    const hipError_t e = HIP_TRY(hipMemsetAsync(ws, 0, kPagedWsBytes, h->stream));  // its item counters
+    const hipError_t e = HIP_TRY(launch_paged_clear(plain(h), ws));
     if (e != hipSuccess) {
         (void)hipFree(ws);
         return fail(h, "paged_reserve: %s failed: %s", failed_call(), hipGetErrorString(e));
@@ -1729,7 +1732,8 @@ int rbt_hip_paged_plan_dev(rbt_hip *h, const rbt_paged_plan *plan) {
     if (!check_paged_plan(h, plan)) return 0;
     if (!h) return fail(nullptr, "paged_plan: handle is NULL");
     if (!set_device(h)) return 0;
-    HIP_OK(h, launch_paged_plan(lc(h, kProfPagedPlan), plain(h), *plan));
+    HIP_OK(h, launch_paged_plan(lc(h, kProfPagedPlan), *plan));
+    if (plan->max_tokens > kPlanRowsInOne) HIP_OK(h, launch_paged_plan_rows(lc(h, kProfPagedRows), *plan));
     return prof_collect(h);
 }
 
@@ -1752,8 +1756,23 @@ int rbt_hip_paged_attn_dev(rbt_hip *h, const rbt_paged_kv *kv, const rbt_paged_b
     const uint64_t qd = (uint64_t)n_heads * (uint64_t)kv->head_dim;
     const float sc = scale == 0.0f ? 1.0f / sqrtf((float)kv->head_dim) : scale;
     if (!paged_ws_reserve(h)) return 0;
-    HIP_OK(h, launch_paged_attn(lc(h, kProfPagedAttn), plain(h), *kv, *batch, q, q_stride ? q_stride : qd, T, n_heads, sc,
-                                window, out, out_stride ? out_stride : qd, h->paged_ws));
+    const PagedAttn p{*kv, *batch, q, q_stride ? q_stride : qd, T, n_heads, sc, window, out, out_stride ? out_stride : qd,
+                      h->paged_ws};
+    if (!paged_attn_tiled(p)) {
+        HIP_OK(h, launch_paged_attn(lc(h, kProfPagedAttn), p));
+        return prof_collect(h);
+    }
+    bool stale = h->paged_ws_stale;
+    if (stale) {  // clear the workspace; in a graph that is being captured that has not happened yet
+        hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+        HIP_OK(h, hipStreamIsCapturing(h->stream, &cap));
+        HIP_OK(h, launch_paged_clear(plain(h), h->paged_ws));
+        stale = cap != hipStreamCaptureStatusNone;
+    }
+    HIP_OK(h, launch_paged_attn(lc(h, kProfPagedAttn), p));
+    h->paged_ws_stale = true;  // until its merge is launched too
+    HIP_OK(h, launch_paged_merge(lc(h, kProfPagedMerge), p));
+    h->paged_ws_stale = stale;
     return prof_collect(h);
 }
 

@@ -16,6 +16,7 @@ namespace rbt {
 constexpr int kPagedMaxReq = 4096;   // requests of a step: their prefix sums sit in LDS
 constexpr int kPagedMaxHd = 256;
 constexpr int kPagedMaxLen = 0x7FFFFC00;  // positions of a request's table
+constexpr int kPlanRowsInOne = 2048;  // rows up to which the plan is one launch
 constexpr size_t kPagedWsBytes = 128u << 20;  // the attention's workspace
 
 // n / d for 0 <= n < 2^31 as a product: with s = ceil(log2 d) and m = floor(2^32 (2^s - d) / d) + 1,

@@ -152,8 +152,9 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a, int rows
 }
 
 __global__ __launch_bounds__(256) void plan_rows_kernel(PlanArgs a) {
-    const int t = blockIdx.x * 256 + threadIdx.x;
-    if (t >= a.max_tokens) return;
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (id >= a.max_tokens) return;
+    const int t = (int)id;
     if (t >= a.q_start[a.n_req]) {
         a.slots[t] = a.positions[t] = -1;
         return;
@@ -1317,8 +1318,8 @@ __device__ __forceinline__ void attn_thin(const AttnArgs &a, int block, int bloc
         if (x.k0 < x.k1) tab.ask(a, x.r, x.k0, x.k0 + min(span, x.k1 - x.k0));
         // fn(w0, w1, page0, bad) over the stretches of the piece that the table holds
         auto stretches = [&](auto fn) {
-            for (int w0 = x.k0; w0 < x.k1; w0 += span) {
-                const int w1 = min(x.k1, w0 + min(span, x.k1 - w0));
+            for (int w0 = x.k0, w1; w0 < x.k1; w0 = w1) {
+                w1 = w0 + min(span, x.k1 - w0);
                 if (w0 != x.k0) tab.ask(a, x.r, w0, w1);
                 const bool bad = tab.fill(a, s_tab);
                 fn(w0, w1, (int)page_of((uint32_t)w0, a.d.div), bad);
@@ -1467,8 +1468,9 @@ __device__ __forceinline__ void attn_wide(const AttnArgs &a, int block, int bloc
         PageTab<DT> tab;
         if (x.k0 < x.k1) tab.ask(a, x.r, x.k0, x.k0 + min(span, x.k1 - x.k0));
         wave_init(w, a, x.q, x.cut.rows, x.kvh, wr0, Sh::Q_AT + 32 * wv * PaddedTile<HDP>::ROW);
-        for (int w0 = x.k0; w0 < x.k1; w0 += span) {
-            const int w1 = min(x.k1, w0 + min(span, x.k1 - w0)), page0 = (int)page_of((uint32_t)w0, a.d.div);
+        for (int w0 = x.k0, w1; w0 < x.k1; w0 = w1) {
+            w1 = w0 + min(span, x.k1 - w0);
+            const int page0 = (int)page_of((uint32_t)w0, a.d.div);
             if (w0 != x.k0) tab.ask(a, x.r, w0, w1);
             const bool bad = tab.fill(a, s_tab);
             // the wave's part of 32 staged positions from j on: whether it has any
@@ -1663,6 +1665,11 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(AttnArgs a) {
             merge_block<HDP, false>(a, hw, id - nt, s_state, s_o);
 }
 
+__global__ void attn_clear_kernel(uint8_t *ws) {
+    if (threadIdx.x < 8)
+        AttnWs<false>::header(ws)->taken[threadIdx.x][0] = AttnWs<true>::header(ws)->taken[threadIdx.x][0] = 0;
+}
+
 PagedDims dims_of(const rbt_paged_kv &kv) {
     PagedDims d;
     d.n_blocks = kv.n_blocks;
@@ -1677,9 +1684,8 @@ PagedDims dims_of(const rbt_paged_kv &kv) {
 
 }  // namespace
 
-constexpr int kPlanRowsInOne = 2048;  // rows up to which the plan is one launch
-
-hipError_t launch_paged_plan(const Launch &L, const Launch &Lr, const rbt_paged_plan &p) {
+namespace {
+PlanArgs plan_args(const rbt_paged_plan &p) {
     PlanArgs a;
     a.n_req = p.n_req;
     a.max_blocks = p.max_blocks;
@@ -1697,10 +1703,15 @@ hipError_t launch_paged_plan(const Launch &L, const Launch &Lr, const rbt_paged_
     a.slots = p.slots;
     a.positions = p.positions;
     a.status = p.status;
-    const int rows = p.max_tokens <= kPlanRowsInOne;
-    const hipError_t e = launch(L, plan_kernel, dim3(1), dim3(kPlanThreads), 0, a, rows);
-    if (e != hipSuccess || rows) return e;
-    return launch(Lr, plan_rows_kernel, dim3((unsigned)((p.max_tokens + 255) / 256)), dim3(256), 0, a);
+    return a;
+}
+}  // namespace
+
+hipError_t launch_paged_plan(const Launch &L, const rbt_paged_plan &p) {
+    return launch(L, plan_kernel, dim3(1), dim3(kPlanThreads), 0, plan_args(p), (int)(p.max_tokens <= kPlanRowsInOne));
+}
+hipError_t launch_paged_plan_rows(const Launch &L, const rbt_paged_plan &p) {
+    return launch(L, plan_rows_kernel, dim3((unsigned)(((int64_t)p.max_tokens + 255) / 256)), dim3(256), 0, plan_args(p));
 }
 
 hipError_t launch_paged_append(const Launch &L, const rbt_paged_kv &kv, const rbt_paged_rows &w) {
@@ -1741,6 +1752,30 @@ hipError_t launch_paged_append(const Launch &L, const rbt_paged_kv &kv, const rb
 }
 
 namespace {
+AttnArgs attn_args(const PagedAttn &p) {
+    AttnArgs a;
+    a.d = dims_of(p.kv);
+    a.n_req = p.batch.n_req;
+    a.max_blocks = p.batch.max_blocks;
+    a.T = p.T;
+    a.n_heads = p.n_heads;
+    a.window = p.window;
+    a.group = page_div(p.n_heads / p.kv.n_kv_heads);
+    a.thin = a.wide = 0;
+    a.scale2 = p.scale * 1.44269504088896340736f;
+    a.tables = p.batch.tables;
+    a.kv_len = p.batch.kv_len;
+    a.q_start = p.batch.q_start;
+    a.kc = p.kv.k;
+    a.vc = p.kv.v;
+    a.q = p.q;
+    a.out = p.out;
+    a.q_stride = p.q_stride;
+    a.out_stride = p.out_stride;
+    a.ws = static_cast<uint8_t *>(p.ws);
+    return a;
+}
+
 // LDS past 64 KiB has to be asked for, once per kernel and device.
 template <typename F>
 hipError_t ask_lds(F kernel, int bytes, std::atomic<uint64_t> &asked) {
@@ -1755,64 +1790,62 @@ hipError_t ask_lds(F kernel, int bytes, std::atomic<uint64_t> &asked) {
     return f;
 }
 
+// Which blocks a call has, and their LDS. Requests of up to 16 rows have blocks of their own, where their tiles and the
+// step's prefix sums fit LDS (a bf16 cache with head dims above 128: up to 2500 requests). Blocks that no request can
+// belong to are left out; otherwise each kind finds its requests on the device.
 template <int DT, int HDP>
-hipError_t launch_attn(const Launch &L, const Launch &Lm, AttnArgs a) {
+int attn_blocks(AttnArgs &a) {
     using Sh = AttnShape<DT, HDP>;
     const int G = a.n_heads / a.d.n_kv;
-    // Requests of up to 16 rows have blocks of their own, where their tiles and the step's prefix sums fit LDS (a bf16
-    // cache with head dims above 128: up to 2500 requests). Blocks that no request can belong to are left out;
-    // otherwise each kind finds its requests on the device.
     a.thin = G <= kThinRows && attn_lds(Sh::TILE, a.n_req) <= kLdsBytes;
     a.wide = !a.thin || (int64_t)a.T * G > kThinRows;
-    const int lds = attn_lds(a.thin ? Sh::TILE : WideShape<DT, HDP>::TILE, a.n_req);
     static_assert(attn_lds(WideShape<DT, HDP>::TILE, kPagedMaxReq) <= kLdsBytes, "wide blocks take any step");
+    return attn_lds(a.thin ? Sh::TILE : WideShape<DT, HDP>::TILE, a.n_req);
+}
+template <int DT, int HDP>
+hipError_t launch_attn(const Launch &L, AttnArgs a, bool merge) {
+    using Sh = AttnShape<DT, HDP>;
+    const int lds = attn_blocks<DT, HDP>(a);
+    if (merge) return launch(L, attn_merge_kernel<HDP>, dim3(1024), dim3(256), 0, a);
     static std::atomic<uint64_t> asked{0};
-    hipError_t e = ask_lds(attn_kernel<DT, HDP>, kLdsBytes, asked);
-    if (e == hipSuccess)
-        e = launch(L, attn_kernel<DT, HDP>, dim3((unsigned)(Sh::BLOCKS * (a.wide + a.thin))), dim3(256), (uint32_t)lds, a);
+    const hipError_t e = ask_lds(attn_kernel<DT, HDP>, kLdsBytes, asked);
     if (e != hipSuccess) return e;
-    return launch(Lm, attn_merge_kernel<HDP>, dim3(1024), dim3(256), 0, a);
+    return launch(L, attn_kernel<DT, HDP>, dim3((unsigned)(Sh::BLOCKS * (a.wide + a.thin))), dim3(256), (uint32_t)lds, a);
+}
+hipError_t launch_tiled(const Launch &L, const PagedAttn &p, bool merge) {
+    const AttnArgs a = attn_args(p);
+    const int hd = a.d.hd;
+    if (p.kv.dtype == RBT_DT_BF16)
+        return hd <= 64 ? launch_attn<RBT_DT_BF16, 64>(L, a, merge)
+                        : hd <= 128 ? launch_attn<RBT_DT_BF16, 128>(L, a, merge) : launch_attn<RBT_DT_BF16, 256>(L, a, merge);
+    return hd <= 64 ? launch_attn<RBT_DT_F32, 64>(L, a, merge)
+                    : hd <= 128 ? launch_attn<RBT_DT_F32, 128>(L, a, merge) : launch_attn<RBT_DT_F32, 256>(L, a, merge);
 }
 }  // namespace
 
-hipError_t launch_paged_attn(const Launch &L, const Launch &Lm, const rbt_paged_kv &kv, const rbt_paged_batch &b,
-                             const float *q, uint64_t q_stride, int T, int n_heads, float scale, int window, float *out,
-                             uint64_t out_stride, void *ws) {
-    if (T < 1 || b.n_req < 1) return hipSuccess;
-    AttnArgs a;
-    a.d = dims_of(kv);
-    a.n_req = b.n_req;
-    a.max_blocks = b.max_blocks;
-    a.T = T;
-    a.n_heads = n_heads;
-    a.group = page_div(n_heads / kv.n_kv_heads);
-    a.window = window;
-    a.scale2 = scale * 1.44269504088896340736f;
-    a.tables = b.tables;
-    a.kv_len = b.kv_len;
-    a.q_start = b.q_start;
-    a.kc = kv.k;
-    a.vc = kv.v;
-    a.q = q;
-    a.out = out;
-    a.q_stride = q_stride;
-    a.out_stride = out_stride;
-    a.ws = static_cast<uint8_t *>(ws);
-    const auto a16 = [](const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
-    const int esz = kv.dtype == RBT_DT_BF16 ? 2 : 4;
-    if (kv.head_dim % 8 == 0 && a16(q) && a16(out) && a16(kv.k) && a16(kv.v) && q_stride % 4 == 0 && out_stride % 4 == 0 &&
-        a.d.block_stride * esz % 16 == 0) {
-        const int hdp = kv.head_dim <= 64 ? 64 : kv.head_dim <= 128 ? 128 : 256;
-        if (kv.dtype == RBT_DT_BF16)
-            return hdp == 64 ? launch_attn<RBT_DT_BF16, 64>(L, Lm, a)
-                             : hdp == 128 ? launch_attn<RBT_DT_BF16, 128>(L, Lm, a) : launch_attn<RBT_DT_BF16, 256>(L, Lm, a);
-        return hdp == 64 ? launch_attn<RBT_DT_F32, 64>(L, Lm, a)
-                         : hdp == 128 ? launch_attn<RBT_DT_F32, 128>(L, Lm, a) : launch_attn<RBT_DT_F32, 256>(L, Lm, a);
-    }
-    const uint64_t rows = (uint64_t)T * (uint64_t)n_heads;
+// On the matrix cores: 16-byte loads everywhere, offsets within a block in 32 bits.
+bool paged_attn_tiled(const PagedAttn &p) {
+    const PagedDims d = dims_of(p.kv);
+    const auto a16 = [](const void *x) { return (reinterpret_cast<uintptr_t>(x) & 15u) == 0; };
+    const uint64_t esz = p.kv.dtype == RBT_DT_BF16 ? 2 : 4;
+    return d.hd % 8 == 0 && a16(p.q) && a16(p.out) && a16(p.kv.k) && a16(p.kv.v) && p.q_stride % 4 == 0 &&
+           p.out_stride % 4 == 0 && d.block_stride * esz % 16 == 0 &&
+           (uint64_t)d.n_kv * (uint64_t)d.block_size * (uint64_t)d.hd * esz <= UINT32_MAX;
+}
+
+hipError_t launch_paged_attn(const Launch &L, const PagedAttn &p) {
+    if (paged_attn_tiled(p)) return launch_tiled(L, p, false);
+    const AttnArgs a = attn_args(p);
+    const uint64_t rows = (uint64_t)p.T * (uint64_t)p.n_heads;
     const dim3 g((unsigned)(rows < 65536 ? rows : 65536));
-    return kv.dtype == RBT_DT_BF16 ? launch(L, attn_any_kernel<RBT_DT_BF16>, g, dim3(256), 0, a)
-                                   : launch(L, attn_any_kernel<RBT_DT_F32>, g, dim3(256), 0, a);
+    return p.kv.dtype == RBT_DT_BF16 ? launch(L, attn_any_kernel<RBT_DT_BF16>, g, dim3(256), 0, a)
+                                     : launch(L, attn_any_kernel<RBT_DT_F32>, g, dim3(256), 0, a);
+}
+
+hipError_t launch_paged_merge(const Launch &L, const PagedAttn &p) { return launch_tiled(L, p, true); }
+
+hipError_t launch_paged_clear(const Launch &L, void *ws) {
+    return launch(L, attn_clear_kernel, dim3(1), dim3(64), 0, static_cast<uint8_t *>(ws));
 }
 
 }  // namespace rbt

@@ -410,12 +410,30 @@ hipError_t launch_record_routing(const Launch &L, const StepState *st, const int
 
 // ---- the paged key/value cache (paged.hip); the arguments are checked (api.hip)
 // Lr: launch context of the rows' own launch, which large steps take.
-hipError_t launch_paged_plan(const Launch &L, const Launch &Lr, const rbt_paged_plan &p);
+// rows beyond kPlanRowsInOne: launch_paged_plan_rows follows
+hipError_t launch_paged_plan(const Launch &L, const rbt_paged_plan &p);
+hipError_t launch_paged_plan_rows(const Launch &L, const rbt_paged_plan &p);
 hipError_t launch_paged_append(const Launch &L, const rbt_paged_kv &kv, const rbt_paged_rows &w);
 // Strides and scale as given to the kernels (not 0). Lm: launch context of the merge. ws: kPagedWsBytes.
-hipError_t launch_paged_attn(const Launch &L, const Launch &Lm, const rbt_paged_kv &kv, const rbt_paged_batch &b,
-                             const float *q, uint64_t q_stride, int T, int n_heads, float scale, int window, float *out,
-                             uint64_t out_stride, void *ws);
+// One attention call, strides in floats. Calls on the matrix cores (paged_attn_tiled) leave partial results and item
+// counters in ws, which launch_paged_merge joins and clears; where it could not be launched, launch_paged_clear has to
+// be before the next call.
+struct PagedAttn {
+    rbt_paged_kv kv;
+    rbt_paged_batch batch;
+    const float *q;
+    uint64_t q_stride;
+    int T, n_heads;
+    float scale;
+    int window;
+    float *out;
+    uint64_t out_stride;
+    void *ws;
+};
+bool paged_attn_tiled(const PagedAttn &p);
+hipError_t launch_paged_attn(const Launch &L, const PagedAttn &p);
+hipError_t launch_paged_merge(const Launch &L, const PagedAttn &p);
+hipError_t launch_paged_clear(const Launch &L, void *ws);
 
 // Dense matvec (one row per wave).
 hipError_t launch_matvec(const Launch &L, int dtype, const void *W, const float *x, float *out, int rows, int cols);

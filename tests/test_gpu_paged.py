@@ -2,15 +2,19 @@
 64 bits on the host: the plan's whole numbers exactly, floats within bounds that follow from the arithmetic.
 
 Attention: with the engine's formulas in f32, a score q.k * scale of hd products is off by at most about sqrt(hd) *
-2^-24 of the sum of their magnitudes A (sums in any order), plus a few rounded steps of the exponent, and a weight
-by that much relatively; in the products with v a weight keeps at least 16 bits (2^-17). The output, a mean of
-values under weights that are each off by a relative w, and whose sum is off by no more, is off by at most 2 w
-max|v|. f32 sums over n positions add about sqrt(n) 2^-24.
+2^-24 of the sum of their magnitudes A (sums in any order), plus four steps more (the scaled query, the exponent's
+difference, the products of parts below 2^-24), and a weight by that much relatively; its power and its products add a
+few steps of 2^-24 each (16), sums over n positions sqrt(n). The output, a mean of values under weights that are each
+off by a relative w, and whose sum is off by no more, is off by at most 2 w max|v|.
 
 Append: a norm is a sum of n squares (sqrt(n) 2^-24 of it, half of that in the root) and three rounded
 products; RoPE adds two products and a sum; a cache of bf16 is off by at most half a step, 2^-8 of the value.
 """
 import ctypes as C
+import json
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -241,7 +245,8 @@ def rope_table(n, hd):
 # tokens, heads, kv heads, head dim, block, dtype, norm, rope, extra floats per row
 APPENDS = [(1, 16, 16, 128, 16, BF16, 1, 1, 0), (5, 4, 2, 64, 8, BF16, 1, 1, 0), (33, 6, 2, 80, 24, F32, 0, 1, 0),
            (7, 3, 1, 20, 5, BF16, 1, 1, 3), (9, 5, 5, 7, 3, F32, 1, 0, 1), (130, 8, 1, 256, 32, BF16, 0, 0, 0),
-           (300, 16, 16, 128, 16, F32, 1, 1, 256), (40, 2, 2, 1, 1, BF16, 1, 0, 0), (64, 12, 4, 96, 16, BF16, 1, 1, 4)]
+           (300, 16, 16, 128, 16, F32, 1, 1, 256), (21, 32, 32, 128, 16, BF16, 1, 1, 0), (6, 17, 1, 128, 8, F32, 1, 1, 64),
+           (3, 65, 5, 128, 4, BF16, 1, 1, 0), (2, 40, 40, 128, 16, F32, 0, 1, 8), (40, 2, 2, 1, 1, BF16, 1, 0, 0), (64, 12, 4, 96, 16, BF16, 1, 1, 4)]
 
 
 @pytest.mark.parametrize("q_in", ["q", "in place", "no q"])
@@ -420,7 +425,7 @@ class Step:
                 A = max(A, float((np.abs(q[:, h]) @ np.abs(kf).T).max() * abs(sc)))
                 vmax = max(vmax, float(np.abs(np.where(np.isfinite(v), v, 0.0)).max()))
             nmax = max(nmax, tot)
-        w = 2.0**-17 + 2.0**-24 * (hd**0.5 * A + nmax**0.5 + 8)
+        w = 2.0**-24 * ((hd**0.5 + 4) * A + nmax**0.5 + 16)
         return out.reshape(self.T, self.qd), 2 * w * vmax
 
     def check(self, dev, scale=0.0, window=0, unseen=None):
@@ -572,6 +577,342 @@ def test_attention_of_many_requests(dev, up):
     rng = np.random.default_rng(13)
     lens = [(int(rng.integers(0, 60)), int(rng.integers(0, 3))) for _ in range(4096)]
     Step(up, lens, 1, 1, 64, 16, BF16, seed=14).upload().check(dev)
+
+
+# ---------------------------------------------------------------- cut ranges, large caches
+# (cached, new) of requests whose positions are cut into pieces that several blocks take
+CUT = [(1300, 100), (2500, 1), (700, 0), (900, 2)]
+CUT_SHAPES = [(2, 2, 128, 16, BF16), (4, 2, 64, 24, F32), (4, 4, 256, 8, BF16), (3, 1, 72, 1, F32)]
+CUT_IDS = ["bf16", "f32", "256", "72"]
+
+
+@pytest.mark.parametrize("window", [0, 300, 1024])
+@pytest.mark.parametrize("shape", CUT_SHAPES, ids=CUT_IDS)
+def test_attention_of_cut_ranges(dev, up, shape, window):
+    """Pieces, some of whose pages lie outside the cache, a whole piece's among them; values that are not finite are
+    seen by some rows of a tile. The same call again gives the same bits."""
+    s = Step(up, CUT, *shape, seed=21)
+    bs = s.bs
+    for r, lo, hi in ((0, 256, 640), (1, 1024, 1300), (3, 0, 130), (1, 2450, 2451)):
+        s.tables[r, lo // bs:hi // bs + 1] = -1
+    bad = lambda r, j: not 0 <= s.tables[r, j // bs] < s.nb  # noqa: E731
+    for r, at, d, x in ((0, 1350, 3, np.inf), (0, 700, 5, np.nan), (1, 2000, 2, -np.inf)):
+        s.v[r][at, :, d] = x
+        s.dense[1, s.tables[r, at // bs], :, at % bs, d] = x
+    got = s.upload().run(dev, window=window)
+    want, tol = s.reference(window=window, unseen=bad)
+    fin = np.isfinite(want)
+    out = got[:, :s.qd]
+    assert np.array_equal(np.isfinite(out), fin) and np.array_equal(np.isnan(out), np.isnan(want))
+    assert np.abs(out[fin] - want[fin]).max() <= tol
+    assert s.run(dev, window=window).tobytes() == got.tobytes()
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("new", [1, 24])
+def test_attention_over_more_pages_than_a_table_holds(dev, up, dt, new):
+    """Blocks of one position: a piece of a large step lies on more pages than are looked up at a time."""
+    lens = [(1500 + 9 * r, new) for r in range(24)]
+    s = Step(up, lens, 16, 16, 8, 1, dt, seed=22)
+    for r in range(0, 24, 5):
+        s.tables[r, 600:603] = (-1, s.nb, 2**31 - 1)
+    s.upload().check(dev, unseen=lambda r, j: not 0 <= s.tables[r, j] < s.nb)
+    s.check(dev, window=1400, unseen=lambda r, j: not 0 <= s.tables[r, j] < s.nb)
+
+
+def test_attention_of_many_requests_of_large_heads(dev, up):
+    """More requests than leave room in LDS for the tiles of decoding rows: the wide tiles take them."""
+    rng = np.random.default_rng(23)
+    lens = [(int(rng.integers(0, 40)), int(rng.integers(0, 3))) for _ in range(3000)]
+    Step(up, lens, 1, 1, 256, 16, BF16, seed=24).upload().check(dev)
+
+
+def append_and_attend(dev, up, kv, H, tables, max_blocks, n, seed):
+    """n new positions of one request through append and attention: (outputs, what they have to be, tolerance)."""
+    KV, hd, bs = kv.n_kv_heads, kv.head_dim, kv.block_size
+    x = np.random.default_rng(seed).standard_normal((n, (H + 2 * KV) * hd)).astype(np.float32)
+    row, pos = x.shape[1], np.arange(n)
+    slots = (tables[pos // bs].astype(np.int64) * bs + pos % bs).astype(np.int32)
+    d_x, d_o = up.up(x), up.up(np.full((n, H * hd), -5.0, np.float32))
+    dev.paged_append(kv, hip.paged_rows_desc(n, H, None, C.c_void_p(d_x.ptr + 4 * H * hd),
+                                             C.c_void_p(d_x.ptr + 4 * (H + KV) * hd), None, None, up.up(slots),
+                                             k_stride=row, v_stride=row))
+    t = np.full(max_blocks, -1, np.int32)
+    t[:len(tables)] = tables
+    b = hip.paged_batch_desc(1, max_blocks, up.up(t), up.up(np.array([n], np.int32)), up.up(np.array([0, n], np.int32)))
+    dev.paged_attn(kv, b, d_x, n, H, d_o, q_stride=row)
+    ref = Step(up, [(0, n)], H, KV, hd, bs if bs < 4096 else 16, kv.dtype)
+    ref.q = x[:, :H * hd]
+    ref.k, ref.v = ([to_cache(x[:, i * hd:(i + KV) * hd], kv.dtype)[1].reshape(n, KV, hd)] for i in (H, H + KV))
+    return dev.d2h(d_o, (n, H * hd), np.float32), *ref.reference()
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("hd", [128, 20])
+def test_cache_beyond_32_bits(dev, up, dt, hd):
+    """Blocks whose elements lie past 2^32, in the caches' middle and at their end."""
+    esz, KV, bs = (4, 2)[dt == BF16], 4, 16
+    block = KV * bs * hd
+    stride = (1 << 20) + 8 * 128  # elements between blocks
+    nb = (1 << 32) // stride + 40
+    size = ((nb - 1) * stride + block) * esz
+    k, v = dev.malloc(size), dev.malloc(size)
+    try:
+        kv = hip.paged_kv_desc(nb, bs, KV, hd, dt, k, v, stride)
+        tables = np.array([nb - 1, 3, nb - 2, nb // 2, 0, nb - 40], np.int32)
+        got, want, tol = append_and_attend(dev, up, kv, 8, tables, 6, 90, 25)
+        assert np.abs(got - want).max() <= tol
+    finally:
+        dev.free(k)
+        dev.free(v)
+
+
+@pytest.mark.parametrize("bs", [1 << 20, (1 << 22) + 1])
+def test_blocks_around_4_gib(dev, up, bs):
+    """A block just below 4 GiB, whose last head's rows lie past 2^31 bytes, and one beyond."""
+    KV, hd = 15, 128
+    if bs > 1 << 20:
+        KV = 4
+    k, v = dev.malloc(2 * KV * bs * hd), dev.malloc(2 * KV * bs * hd)
+    try:
+        kv = hip.paged_kv_desc(1, bs, KV, hd, BF16, k, v)
+        got, want, tol = append_and_attend(dev, up, kv, KV, np.zeros(1, np.int32), 1, 70, 26)
+        assert np.abs(got - want).max() <= tol
+    finally:
+        dev.free(k)
+        dev.free(v)
+
+
+@pytest.mark.parametrize("shape", [(2, 2, 128, 16, BF16), (4, 1, 64, 16, F32), (3, 1, 20, 5, BF16)], ids=["bf16", "f32", "20"])
+def test_attention_in_place(dev, up, shape):
+    """out may be q: a cut tile's pieces and rows that are computed again read q before it is written."""
+    s = Step(up, [(900, 60), (40, 1), (0, 20)], *shape, seed=27)
+    s.v[0][930, :, 1] = np.inf
+    s.dense[1, s.tables[0, 930 // s.bs], :, 930 % s.bs, 1] = np.inf
+    want = s.upload().run(dev)[:, :s.qd]
+    dev.paged_attn(s.kv, s.batch, s.d_q, s.rows, s.H, s.d_q)
+    assert dev.d2h(s.d_q, (s.rows, s.qd), np.float32).tobytes() == want.tobytes()
+
+
+# ---------------------------------------------------------------- graphs, handles, failures
+class Graph:
+    """What fn launches on the handle's stream, captured."""
+    L = None
+
+    def __init__(self, dev, fn):
+        if Graph.L is None:
+            L = Graph.L = C.CDLL("libamdhip64.so")
+            L.hipStreamBeginCapture.argtypes = [C.c_void_p, C.c_int]
+            L.hipStreamEndCapture.argtypes = [C.c_void_p, C.POINTER(C.c_void_p)]
+            L.hipGraphInstantiate.argtypes = [C.POINTER(C.c_void_p), C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t]
+            L.hipGraphLaunch.argtypes = [C.c_void_p, C.c_void_p]
+            L.hipGraphExecDestroy.argtypes = L.hipGraphDestroy.argtypes = [C.c_void_p]
+        self.dev, self.graph, self.exec = dev, C.c_void_p(), C.c_void_p()
+        assert self.L.hipStreamBeginCapture(dev.stream, 2) == 0
+        try:
+            fn()
+        finally:
+            assert self.L.hipStreamEndCapture(dev.stream, C.byref(self.graph)) == 0
+        assert self.L.hipGraphInstantiate(C.byref(self.exec), self.graph, None, None, 0) == 0
+
+    def replay(self):
+        assert self.L.hipGraphLaunch(self.exec, self.dev.stream) == 0
+
+    def free(self):
+        self.L.hipGraphExecDestroy(self.exec)
+        self.L.hipGraphDestroy(self.graph)
+
+
+class Pool:
+    """The buffers of a serving step (plan, append, attention) on `nb` blocks."""
+
+    def __init__(self, dev, up, R, P, nb, M, H=4, KV=2, hd=64, bs=8, dt=BF16):
+        self.dev, self.M, self.nb, self.H, self.hd, self.R = dev, M, nb, H, hd, R
+        ints = lambda *s: up.up(np.full(s, -1, np.int32))  # noqa: E731
+        self.len, self.t, self.nf = up.up(np.zeros(R, np.int32)), ints(R, P), ints(1)
+        self.free, self.new, qs, sl, pos, self.st = ints(nb), ints(R), ints(R + 1), ints(M), ints(M), ints(1)
+        esz = np.float32 if dt == F32 else np.uint16
+        self.k, self.v = (up.up(np.zeros((nb, KV, bs, hd), esz)) for _ in range(2))
+        self.row = (H + 2 * KV) * hd
+        self.x, self.q, self.o = (up.up(np.zeros((M, n), np.float32)) for n in (self.row, H * hd, H * hd))
+        self.plan = hip.paged_plan_desc(R, P, nb, bs, M, self.len, self.new, self.t, self.free, self.nf, self.len, self.nf,
+                                        qs, sl, pos, self.st)
+        self.kv = hip.paged_kv_desc(nb, bs, KV, hd, dt, self.k, self.v)
+        self.rows = hip.paged_rows_desc(M, H, self.x, C.c_void_p(self.x.ptr + 4 * H * hd),
+                                        C.c_void_p(self.x.ptr + 4 * (H + KV) * hd), self.q, pos, sl,
+                                        rope=up.up(rope_table(P * bs, hd)), n_rope=P * bs, q_stride=self.row,
+                                        k_stride=self.row, v_stride=self.row)
+        self.batch = hip.paged_batch_desc(R, P, self.t, self.len, qs)
+        self.reset()
+
+    def reset(self):
+        self.dev.h2d(self.len, np.zeros(self.R, np.int32))
+        self.dev.h2d(self.free, np.arange(self.nb, dtype=np.int32))
+        self.dev.h2d(self.nf, np.array([self.nb], np.int32))
+
+    def inputs(self, new, seed):
+        self.dev.h2d(self.new, np.array(new, np.int32))
+        self.dev.h2d(self.x, np.random.default_rng(seed).standard_normal((self.M, self.row)).astype(np.float32))
+
+    def step(self, dev=None):
+        d = dev or self.dev
+        d.paged_plan(self.plan)
+        d.paged_append(self.kv, self.rows)
+        d.paged_attn(self.kv, self.batch, self.q, self.M, self.H, self.o)
+
+    def out(self):
+        assert self.dev.d2h(self.st, (1,), np.int32)[0] == 0
+        return self.dev.d2h(self.o, (self.M, self.H * self.hd), np.float32)
+
+
+STEPS = [[600, 0, 17, 1], [1, 40, 20, 1], [1, 1, -1, 1], [70, 1, 60, 1], [-1, 1, 1, 1], [33, 1, 900, 0], [1, 1, 1, 1],
+         [0, 0, 0, 0], [1, -1, -1, 1], [9, 80, 2, 5]]
+
+
+@pytest.mark.parametrize("M", [1000, 2500])
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_a_captured_step_replays_for_other_lengths(dev, up, dt, M):
+    """One graph of plan, append and attention over steps of other lengths, with eager steps of another pool between
+    its replays: each gives the eager step's bits."""
+    dev.paged_reserve()
+    pool, other = Pool(dev, up, 4, 160, 300, M, dt=dt), Pool(dev, up, 4, 160, 300, M, H=8, KV=1, dt=dt)
+    eager = []
+    for i, new in enumerate(STEPS):
+        pool.inputs(new, 40 + i)
+        pool.step()
+        eager.append(pool.out().tobytes())
+    pool.reset()
+    g = Graph(dev, pool.step)
+    try:
+        dev.memset(pool.o, 0)
+        dev.memset(pool.t, 0xFF)
+        for i, new in enumerate(STEPS):
+            pool.inputs(new, 40 + i)
+            other.inputs(STEPS[-1 - i] if min(STEPS[-1 - i]) >= 0 else STEPS[0], i)
+            if i % 2:
+                other.step()
+            g.replay()
+            if i % 3:
+                other.step()
+            dev.synchronize()
+            assert pool.out().tobytes() == eager[i], i
+            other.reset()
+    finally:
+        g.free()
+
+
+def test_two_graphs_of_a_handle_share_its_workspace(dev, up):
+    """Replayed in turn, as the handle's stream orders them."""
+    dev.paged_reserve()
+    steps = [Step(up, CUT, 2, 2, 128, 16, BF16, seed=31).upload(), Step(up, [(2000, 40), (0, 1)], 8, 2, 64, 16, F32, seed=32).upload()]
+    want = [s.run(dev).tobytes() for s in steps]
+    graphs = [Graph(dev, lambda s=s: s.call(dev)) for s in steps]
+    try:
+        for i in range(4):
+            for s in steps:
+                dev.memset(s.d_o, 0)
+            for g in graphs[::1 if i % 2 else -1]:
+                g.replay()
+            dev.synchronize()
+            for s, w in zip(steps, want):
+                got = dev.d2h(s.d_o, (s.rows, s.out_row), np.float32)
+                assert got.tobytes() == w
+    finally:
+        for g in graphs:
+            g.free()
+
+
+def test_capture_before_the_workspace_is_refused():
+    with hip.Device(0) as own:
+        a = Arrays(own)
+        try:
+            s = Step(a, [(30, 8)], 2, 2, 128, 16, BF16, seed=33).upload()
+            none = hip.paged_rows_desc(1, 2, None, s.d_q, s.d_q, None, None, a.up(np.array([-1], np.int32)))
+
+            def call():
+                with pytest.raises(hip.HipError, match="captured before rbt_hip_paged_reserve"):
+                    s.call(own)
+                own.paged_append(s.kv, none)
+            Graph(own, call).free()
+            s.check(own)
+        finally:
+            a.free()
+
+
+def test_two_handles_on_one_cache(dev, up):
+    """Calls of two handles, each on its own stream and workspace, at once."""
+    s = Step(up, CUT + [(300, 300)], 4, 2, 128, 16, BF16, seed=34).upload()
+    want = s.run(dev).tobytes()
+    with hip.Device(0) as own:
+        o = own.upload_array(np.zeros((s.rows, s.out_row), np.float32))
+        own.paged_reserve()
+        own.synchronize()
+        dev.memset(s.d_o, 0)
+        dev.synchronize()
+        for _ in range(5):
+            s.call(dev)
+            own.paged_attn(s.kv, s.batch, s.d_q, s.rows, s.H, o, q_stride=s.q.shape[1], out_stride=s.out_row)
+        assert own.d2h(o, (s.rows, s.out_row), np.float32).tobytes() == want
+        assert dev.d2h(s.d_o, (s.rows, s.out_row), np.float32).tobytes() == want
+        own.free(o)
+
+
+@pytest.mark.parametrize("mode", [1, 2])
+def test_profile_names(up, mode):
+    with hip.Device(0) as own:
+        a = Arrays(own)
+        try:
+            for M, hd, names in ((1000, 64, {"paged_plan", "paged_append", "paged_attn", "paged_merge"}),
+                                 (2500, 20, {"paged_plan", "paged_rows", "paged_append", "paged_attn"})):
+                pool = Pool(own, a, 4, 160, 300, M, hd=hd)
+                pool.inputs([60, 0, 17, 1], 1)
+                own.profile(mode)
+                pool.step()
+                pool.out()
+                after = {n: own.profile_get(n) for n in sorted(names | {"paged_rows", "paged_merge"})}
+                own.profile(0)
+                for n, (ms, k) in after.items():
+                    assert k == (n in names), n
+                    assert ms > 0.0 or n not in names
+        finally:
+            a.free()
+
+
+CHILD = r"""
+import json, sys
+sys.path.insert(0, sys.argv[1])
+import numpy as np
+from rabbitm2_amd import hip
+from tests.test_gpu_paged import Arrays, Step, CUT, BF16
+res = []
+with hip.Device(0) as dev:
+    a = Arrays(dev)
+    s = Step(a, CUT, 2, 2, 128, 16, BF16, seed=35).upload()
+    for _ in range(3):
+        dev.memset(s.d_o, 0)
+        try:
+            got = s.run(dev)
+            want, tol = s.reference()
+            res.append("ok" if np.abs(got[:s.T] - want).max() <= tol else "wrong")
+        except hip.HipError as e:
+            res.append(str(e))
+    a.free()
+print("RESULT " + json.dumps(res), flush=True)
+"""
+
+
+@pytest.mark.parametrize("fault,text", [("malloc:8", "hipMalloc"), ("launch:1", "launch_paged_clear"),
+                                        ("launch:2", "launch_paged_attn"), ("launch:3", "launch_paged_merge")])
+def test_failures_leave_the_handle_usable(fault, text):
+    """The first call fails (the workspace's allocation, one of the launches) and says so; the next ones are right,
+    also where the failed one left its items counted and its pieces unjoined. (Seven arrays are allocated before.)"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    print(f"child with RBT_HIP_FAULT={fault}", flush=True)
+    r = subprocess.run([sys.executable, "-c", CHILD, root], capture_output=True, text=True, timeout=300, cwd=root,
+                       env=dict(os.environ, RBT_HIP_FAULT=fault))
+    assert r.returncode == 0, r.stderr[-3000:]
+    res = json.loads([ln for ln in r.stdout.splitlines() if ln.startswith("RESULT ")][-1][7:])
+    assert text in res[0] and res[1:] == ["ok", "ok"], res
 
 
 # ---------------------------------------------------------------- a step as it is run

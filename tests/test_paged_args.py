@@ -77,7 +77,7 @@ BAD_ATTN = [dict(b=dict(n_req=-1)), dict(b=dict(n_req=4097)), dict(b=dict(max_bl
             dict(b=dict(max_blocks=1 << 30)), dict(b=dict(tables=None)), dict(b=dict(kv_len=None)),
             dict(b=dict(q_start=None)), dict(T=-1), dict(n_heads=0), dict(n_heads=3), dict(n_heads=1 << 20), dict(q=None),
             dict(out=None), dict(scale=float("nan")), dict(scale=float("inf")), dict(window=-1), dict(q_stride=255),
-            dict(out_stride=255), dict(out_stride=1 << 33)]
+            dict(out_stride=255), dict(out_stride=1 << 33), dict(q_stride=300), dict(out_stride=300)]  # out is q
 
 
 @pytest.mark.parametrize("over", BAD_ATTN, ids=[str(o) for o in BAD_ATTN])
