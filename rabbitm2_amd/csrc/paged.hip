@@ -1117,21 +1117,23 @@ __device__ __forceinline__ Item item_of(const AttnArgs &a, int it, int chunk, co
     return x;
 }
 // An eighth of the items to each XCD (blocks b % 8), so that a head's row tiles read its keys and values through one
-// L2. A block starts with the item of its own number and then takes the next one left of its eighth, then of the other
-// eighths: ask() early, its answer used by next() at the item's end.
+// L2. A block starts with the item of its own number and, where there are more items than blocks, then takes the next
+// one left of its eighth, then of the other eighths: ask() early, its answer used by next() at the item's end.
 struct ItemQueue {
     int it, n, xcd, per;  // it < 0: nothing is left
+    bool more;
     AttnHeader *hdr;
     __device__ __forceinline__ int start(int x) const { return (int)((long long)n * x / 8); }
     __device__ __forceinline__ ItemQueue(int n_items, AttnHeader *header, int block, int blocks)
-        : n(n_items), xcd(block & 7), per(blocks >> 3), hdr(header) {
+        : n(n_items), xcd(block & 7), per(blocks >> 3), more(n_items > blocks), hdr(header) {
         it = start(xcd) + (block >> 3);
         if (it >= start(xcd + 1)) it = -1;
     }
-    __device__ __forceinline__ int ask() const { return threadIdx.x == 0 ? atomicAdd(&hdr->taken[xcd][0], 1) : 0; }
+    __device__ __forceinline__ int ask() const { return more && threadIdx.x == 0 ? atomicAdd(&hdr->taken[xcd][0], 1) : 0; }
     // for all threads
     __device__ __forceinline__ void next(int ticket, int *s_next) {
-        for (;;) {
+        it = -1;
+        while (more) {
             if (threadIdx.x < kWave) {  // the answer, or the first other eighth with any left (its counters only grow)
                 const int x = threadIdx.x & 7;
                 int got = __builtin_amdgcn_readfirstlane(ticket) + start(xcd) + per;
