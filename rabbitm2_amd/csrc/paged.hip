@@ -545,8 +545,8 @@ __device__ __forceinline__ Cut cut_of(const AttnArgs &a, const Request &q, int c
     return c;
 }
 template <bool THIN>
-__device__ __forceinline__ int first_with(const Cut &c, int piece) {  // T(piece), for c0 <= piece < nc
-    return (int)(((long long)piece * c.chunk - c.p0) * c.G / kTileRows<THIN>);
+__device__ __forceinline__ int first_with(const Cut &c, int piece) {  // T(piece), for piece < nc; below 0 before c0
+    return (int)(((long long)piece * c.chunk - c.p0) * c.G >> (THIN ? 4 : 7));
 }
 template <bool THIN>
 __device__ __forceinline__ long long pieces_before(const Cut &c, int t) {
@@ -554,8 +554,9 @@ __device__ __forceinline__ long long pieces_before(const Cut &c, int t) {
     for (int i = c.c0; i < c.nc; ++i) n += max(0, t - first_with<THIN>(c, i));
     return n;
 }
-// Tile t's pieces: n of len positions, equal up to whole tiles of 128 (len <= chunk); the last may be shorter or, where
-// the tile's positions are fewer than S(t), empty.
+// Tile t's pieces: n, of len positions each but the last, which may be shorter or, where the tile's positions are fewer
+// than S(t), empty. Thin tiles' are equal up to whole tiles of 128 (what they take is memory, shared evenly); wide
+// tiles' are whole chunks and a rest.
 struct Pieces {
     int n, len;
 };
@@ -564,7 +565,47 @@ __device__ __forceinline__ Pieces pieces_of(const Cut &c, int t) {
     const uint32_t rows = min((uint32_t)(t + 1) * kTileRows<THIN>, (uint32_t)c.rows);
     const uint32_t span = (uint32_t)max(0, min(c.p0 + (int)((rows + (uint32_t)c.G - 1) / (uint32_t)c.G), c.limit));
     const uint32_t n = max(1u, (span + (uint32_t)(c.chunk - 1)) / (uint32_t)c.chunk);
-    return {(int)n, (int)(((span + n - 1) / n + 127) / 128 * 128)};
+    return {(int)n, THIN ? (int)(((span + n - 1) / n + 127) / 128 * 128) : c.chunk};
+}
+// Item `local` of a head's: its tile and piece, the largest first, so that a queue ends with its smallest. Wide tiles'
+// whole chunks, then the rests: tile t of those with c + 1 pieces has about t - T(c) tiles' rows of positions in its
+// rest, so that the rests in descending order are those of the tiles with t - T(c) >= v for falling v.
+struct TilePiece {
+    int tile, piece;
+};
+template <bool THIN>
+__device__ __forceinline__ TilePiece tile_piece(const Cut &c, int local) {
+    for (int i = c.nc - 1; i >= (THIN ? c.c0 : 1); --i) {
+        const int n = c.nt - (i >= c.c0 ? first_with<THIN>(c, i) : 0);
+        if (local < n) return {c.nt - 1 - local, THIN ? i : i - 1};
+        local -= n;
+    }
+    if (THIN) return {c.nt - 1 - local % c.nt, c.c0 - 1 - local / c.nt};
+    if (c.nc == c.c0) return {c.nt - 1 - local, c.nc - 1};
+    // the tiles of class i (i + 1 pieces) are [from(i), to(i)): how many have t - T(i) >= v
+    auto from = [&](int i) { return i >= c.c0 ? first_with<THIN>(c, i) : 0; };
+    auto to = [&](int i) { return i + 1 < c.nc ? first_with<THIN>(c, i + 1) : c.nt; };
+    auto count = [&](int v) {
+        int n = 0;
+        for (int i = c.c0 - 1; i < c.nc; ++i) n += max(0, to(i) - max(from(i), first_with<THIN>(c, i) + v));
+        return n;
+    };
+    int lo = 0, hi = c.nt - first_with<THIN>(c, c.c0 - 1);  // count(lo) > local >= count(hi)
+    while (hi - lo > 1) {
+        const int mid = (int)(((uint32_t)lo + (uint32_t)hi) >> 1);
+        if (count(mid) > local)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    local -= count(hi);
+    int i = c.c0 - 1;  // of the classes that have a tile at lo
+    for (;; ++i) {
+        const int t = first_with<THIN>(c, i) + lo;
+        if (t >= from(i) && t < to(i) && local-- == 0) break;
+        if (i + 1 == c.nc) break;
+    }
+    return {first_with<THIN>(c, i) + lo, i};
 }
 
 // Rows that a block of the merge launch joins: a few per wave, or where many pieces have to be read, as many as one
@@ -612,7 +653,8 @@ __device__ int schedule(const AttnArgs &a, int block, int blocks, int32_t *s_ite
         return 0;
     }
     work = ((s.work[0] + s.work[1]) + (s.work[2] + s.work[3])) * (float)a.d.n_kv / (float)(2 * blocks);
-    int chunk = (int)fminf(work, 1.0e9f) / 128 * 128 + 128;
+    int chunk = THIN ? (int)fminf(work, 1.0e9f) / 128 * 128 + 128 : (int)fminf(2 * work + 127, 1.0e9f) / 128 * 128;
+    chunk = max(chunk, 128);
     for (;;) {
         int v[3] = {0, 0, 0}, inc[3], before[3], total[3];  // items, partial units, merge blocks
         for (int r = r0; r < r1; ++r) {
@@ -1084,24 +1126,14 @@ __device__ __forceinline__ Item item_of(const AttnArgs &a, int it, int chunk, co
     x.q = request(a, x.r);
     x.cut = cut_of<THIN>(a, x.q, chunk);
     int local = it - __builtin_amdgcn_readfirstlane(s_items[x.r]);
-    // With a multiple of eight heads each eighth of the items has its own heads. The last pieces of the longest tiles
-    // first, the first piece of the shortest last: a queue that ends with its smallest items leaves no block waiting.
+    // With a multiple of eight heads each eighth of the items has its own heads.
     const int hx = a.d.n_kv % 8 == 0 ? a.d.n_kv / 8 : a.d.n_kv;
     const int pieces = (int)pieces_before<THIN>(x.cut, x.cut.nt), group = local / (pieces * hx);
     local -= group * pieces * hx;
     x.kvh = group * hx + local % hx;
     local /= hx;
-    int c = x.cut.nc - 1;
-    for (; c >= x.cut.c0; --c) {
-        const int n = x.cut.nt - first_with<THIN>(x.cut, c);
-        if (local < n) break;
-        local -= n;
-    }
-    if (c < x.cut.c0) {
-        c -= local / x.cut.nt;
-        local %= x.cut.nt;
-    }
-    const int tile = x.cut.nt - 1 - local;
+    const TilePiece tp = tile_piece<THIN>(x.cut, local);
+    const int tile = tp.tile, c = tp.piece;
     x.row0 = tile * tr;
     x.n_rows = min(tr, x.cut.rows - x.row0);
     x.pa = place(a, x.q, x.kvh, x.row0).pos;
