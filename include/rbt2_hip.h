@@ -363,7 +363,8 @@ int rbt_hip_paged_append_dev(rbt_hip *h, const rbt_paged_kv *kv, const rbt_paged
  * rows times scale, rounded once in f32. A position outside the table's length or on a block outside [0, n_blocks) is
  * not seen; a row that sees none is 0; rows of no request (behind the last one's) are left as they are. What lies
  * behind a row's own position, infinities and NaN too, does not reach it. Head dims that are multiples of 8, with
- * 16-byte aligned pointers, strides of a multiple of 16 bytes and blocks below 4 GiB, run on the matrix cores; any others run too, slowly. */
+ * 16-byte aligned pointers, strides of a multiple of 16 bytes and blocks below 4 GiB, run on the matrix cores; any
+ * others run too, slowly. */
 int rbt_hip_paged_attn_dev(rbt_hip *h, const rbt_paged_kv *kv, const rbt_paged_batch *batch, const float *q,
                            uint64_t q_stride, int T, int n_heads, float scale, int window, float *out,
                            uint64_t out_stride);

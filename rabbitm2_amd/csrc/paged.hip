@@ -30,9 +30,10 @@ __device__ __forceinline__ int wave_scan(int v) {
 // ---------------------------------------------------------------- plan
 // One block: three prefix sums over the requests (new rows, blocks needed, blocks given back), then the blocks pushed
 // and popped and the rows' slots, each by its place in those sums (a binary search in LDS), so that one long request
-// costs no more than many short ones. All of it is latency, so a new row's block is taken from the free stack, not from
-// the table entry that another thread is writing. Steps of many rows give those to a launch of their own (1024 requests,
-// 32768 rows: @PLAN@).
+// costs no more than many short ones. It moves a few KB and computes next to nothing: what bounds it is latency, so the
+// sums go by DPP, and a new row's block is taken from the free stack, not from the table entry that another thread is
+// writing. Steps of many rows give those to a launch of their own (1024 requests, 32768 rows: 15 us against 27.5 in one
+// launch; 32 requests take 4.1 us, about a launch's own time).
 constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / kWave, kPlanPer = kPagedMaxReq / kPlanThreads;
 
 struct PlanArgs {
@@ -186,7 +187,8 @@ __device__ __forceinline__ void store_kv(void *p, uint64_t i, float v) {
         static_cast<bf16_t *>(p)[i] = (bf16_t)v;  // to nearest even; NaN stays NaN
 }
 
-// grid (tokens), 256 threads: prompt_rope_kernel's arithmetic (prompt.hip) with the cache rows in pages.
+// grid (tokens), 256 threads: prompt_rope_kernel's arithmetic (prompt.hip) with the cache rows in pages. For any head dim
+// and alignment; append_quads_kernel takes the others.
 template <int DT>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     __shared__ float red[8];
@@ -240,8 +242,9 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
 // The same for head dims that are multiples of 8 and 16-byte aligned rows of up to 256 * 8 * kAppendQ floats of q and
 // 256 * 8 * kAppendK of k: everything is asked for at once (the rows whether or not the token has a slot), held in
 // registers through the norm, and each thread turns whole quads of pairs (elements 4 i .. 4 i + 3 of a head's halves).
+// One pass over memory, which bounds it: 4096 tokens of 16 heads of 128 take 33.5 us, 5.1 TB/s (append_kernel 63 us).
 // Rows of up to 2048 floats (the benchmark's model) take a quarter of the registers, so that four times the blocks share
-// a CU (4096 tokens: 45.8 against @APP@ us).
+// a CU (the same 4096 tokens on the larger rows' kernel: 45.8 us).
 constexpr int kAppendQ = 4, kAppendK = 2;
 __device__ __forceinline__ void store4(float *p, f32x4 v) { *reinterpret_cast<f32x4 *>(p) = v; }
 template <int DT>
@@ -482,7 +485,8 @@ __global__ __launch_bounds__(256) void attn_any_kernel(AttnArgs a) {
 //   wide   128 rows, 32 to a wave; the block's waves share each tile of keys and values
 //   thin   requests of up to 16 rows (a decoding token): each wave takes tiles of 32 positions of its own
 // each kind by blocks of its own, and long ranges are cut into pieces that different blocks take, joined by
-// attn_merge_kernel.
+// attn_merge_kernel. (Joined by a tile's last block instead, thin tiles gain a microsecond and wide ones lose 20, whose
+// few blocks then read what others wrote while the rest of the chip waits.)
 //
 // Products: v_mfma_f32_16x16x32_bf16, transposed so that nothing moves between lanes: S^T = K Q^T leaves lane
 // (c = l % 16, g = l / 16) the scores of query c with keys 4 g + i of two 16-key groups, which as they stand are
@@ -490,7 +494,14 @@ __global__ __launch_bounds__(256) void attn_any_kernel(AttnArgs a) {
 // tile by the transposing LDS read (ds_read_b64_tr_b16: lane c of group g gets column c of rows 4 g .. 4 g + 3).
 //
 // Precision: bf16 keys and values enter exactly. f32 operands are cut into three bf16 parts of 8 bits each (exact: 24
-// bits), and the products of parts down to 2^-24 are taken: three for a bf16 cache, six for an f32 one. Sums, the softmax and its state are f32.
+// bits), and the products of parts down to 2^-24 are taken: three for a bf16 cache, six for an f32 one. Sums, the softmax
+// and its state are f32. Outputs are as far from 64 bits as f32 arithmetic leaves them (3e-7 of their size; two parts
+// would be a third faster and 16 bits).
+//
+// What bounds it: a prompt of 4096 tokens (16 heads of 128, bf16) takes 216 us, three products of 69 GFLOP: 955 TFLOP/s
+// of the matrix cores in all, where a large library product reaches 1166; the attention launch alone runs at 1070, the
+// rest joins pieces. 64 decoding sequences of up to 8192 positions take 216 us, 5.8 TB/s of cache. Small steps are
+// latency: the schedule, pages, queries and first keys one after the other, and two launches (one sequence: 16 us).
 //
 // Not finite: a position that a row does not see has weight 0, but 0 times an infinity is NaN, so rows whose
 // result is not finite are computed again by row_any, which reads seen positions only. Rows past the positions
@@ -500,7 +511,7 @@ constexpr int kTabPages = 512;  // pages whose places are held in LDS at a time
 constexpr int kMaxChunk = kPagedMaxLen;  // positions, a multiple of 128
 static_assert(kMaxChunk % 128 == 0, "whole tiles");
 
-// Workspace: for the wide and the thin launch each a header (chunk length, blocks of merging) and the prefix sums of
+// Workspace: for the wide and the thin blocks each a header (chunk length, blocks of the merge) and the prefix sums of
 // those and of the partial units over the requests, then their partials: units of 16 rows, m [16], l [16],
 // o [16][HDP].
 struct AttnHeader {
@@ -522,7 +533,7 @@ struct AttnWs {
 // spans up to S(t) = min(p0 + ceil((t + 1) tr / G), limit) positions, which grow with t, so that tiles from T(c) =
 // floor((c chunk - p0) G / tr) on have more than c pieces. The first c0 pieces are every tile's (T = 0), nc is the
 // last tile's number, and the tiles before t have pieces_before(t) = sum over c of max(0, t - T(c)) in all.
-// rows 0: not this launch's.
+// rows 0: not of this kind.
 template <bool THIN>
 constexpr int kTileRows = THIN ? kThinRows : kWideRows;
 struct Cut {
@@ -608,16 +619,18 @@ __device__ __forceinline__ TilePiece tile_piece(const Cut &c, int local) {
     return {first_with<THIN>(c, i) + lo, i};
 }
 
-// Rows that a block of the merge launch joins: a few per wave, or where many pieces have to be read, as many as one
+// Rows that a block of attn_merge_kernel joins: a few per wave, or where many pieces have to be read, as many as one
 // wave takes, the pieces dealt to the block's four.
 constexpr int kMergeManyPieces = 16;
 template <int HDP>
 __device__ __forceinline__ int merge_rows(int nc) { return 256 / HDP * (nc >= kMergeManyPieces ? 1 : 4); }
 
-// A launch's items (request, head, row tile, piece), by every block for itself: prefix sums over the requests into
-// s_items [n_req + 1] and s_units. The chunk length spreads the work over about two rounds of blocks; it doubles
-// until the partials fit, which ends at the latest at kMaxChunk, where no tile is cut. Returns 0 where the launch has
-// no request.
+// A kind's items (request, head, row tile, piece), by every block for itself: prefix sums over the requests into
+// s_items [n_req + 1] and s_units. The chunk length: thin, what spreads the positions over two rounds of blocks, evenly;
+// wide, over one, whose gaps the rests of the tiles fill: fewer partials, fewer diagonals (13 prompts and chunks of 200
+// to 4096 tokens: 127 us on average against 132 with chunks of half that; a windowed prompt of 2 x 2048 67 against
+// 108, three prompts of 1500 169 against 141). It doubles until the partials fit, which ends at the latest at kMaxChunk,
+// where no tile is cut. Returns 0 where no request is of this kind.
 struct ScheduleShared {
     float work[4];
     int any[4], sum[4][3];
@@ -627,7 +640,7 @@ __device__ int schedule(const AttnArgs &a, int block, int blocks, int32_t *s_ite
     constexpr int tr = kTileRows<THIN>, kUnits = AttnWs<THIN>::max_units(HDP);
     const int per = (a.n_req + 255) / 256, r0 = min(a.n_req, (int)threadIdx.x * per), r1 = min(a.n_req, r0 + per);
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-    AttnHeader *hdr = block == 0 ? AttnWs<THIN>::header(a.ws) : nullptr;  // one block tells the merge launch
+    AttnHeader *hdr = block == 0 ? AttnWs<THIN>::header(a.ws) : nullptr;  // one block tells attn_merge_kernel
     // the first request of a thread (all of them, up to 256 requests) stays in registers
     Request first{};
     if (r0 < r1) first = request(a, r0);
@@ -801,8 +814,9 @@ struct WaveState {
     PartConsts pc;
 };
 
-// 32 positions, staged from byte k_off (keys) and v_off (values) of LDS on, parts `part` bytes apart; between(i) is called among the products, for i = 0 .. HDP / 16 NP - 1 in turn; seen(n): bit 4 t + i, whether query n of this lane sees key 16 t + 4 g + i of them
-// (asked where !full).
+// 32 positions, staged from byte k_off (keys) and v_off (values) of LDS on, parts `part` bytes apart; between(i) is
+// called among the products, for i = 0 .. HDP / 16 NP - 1 in turn; seen(n): bit 4 t + i, whether query n of this lane
+// sees key 16 t + 4 g + i of them (asked where !full).
 template <int HDP, int NQ, int QP, int NP, int part, typename Tile, typename Between, typename Seen>
 __device__ __forceinline__ void attn_step(WaveState<HDP, NQ, QP> &w, const Tile &tile, int k_off, int v_off, bool full,
                                           Between between, Seen seen) {
@@ -1108,7 +1122,7 @@ __device__ __forceinline__ Place place(const AttnArgs &a, const Request &q, int 
     return {q.t0 + tok, kvh * G + row - tok * G, q.p0 + tok};
 }
 
-// A launch's item.
+// One of them.
 struct Item {
     Request q;
     Cut cut;
@@ -1593,9 +1607,9 @@ __device__ __forceinline__ void attn_wide(const AttnArgs &a, int block, int bloc
     }
 }
 
-// One launch of both: the wide launch's blocks first, which leave at once where no request is theirs; the thin ones
-// fill the places that the last wide ones leave (in launches of their own: prompts and decoding rows mixed 33.6 against
-// @MIX@ us, 32 decoding sequences @DEC@).
+// One launch of both: the wide blocks first, which leave at once where no request is theirs; the thin ones fill the
+// places that the last wide ones leave (prompts and decoding rows mixed: 29.5 us, 33.6 in two launches; 32 decoding
+// sequences: 69.5 and 68.2).
 template <int DT, int HDP>
 struct AttnShape {
     static constexpr int TILE = std::max(WideShape<DT, HDP>::TILE, ThinShape<DT, HDP>::TILE);
