@@ -373,6 +373,19 @@ int rbt_hip_paged_attn_dev(rbt_hip *h, const rbt_paged_kv *kv, const rbt_paged_b
  * first call does otherwise; needed before capturing one. */
 int rbt_hip_paged_reserve(rbt_hip *h);
 
+/* The whole model on a paged cache: steps of up to n_req requests that come, read their prompts in pieces of any
+ * length, decode and end independently (rabbit2.c:453-548 for each of them). paged_init allocates n_layers caches of
+ * n_blocks blocks of block_size positions in dtype (RBT_DT_F32: the engine's cache; RBT_DT_BF16: half the memory, keys
+ * and values rounded) and buffers for steps of max_tokens tokens (up to 65535); ctx as in rbt_hip_state_init, per
+ * request. It ends all requests of an earlier one, and so does another model.
+ * forward_paged runs one step: new_len[r] tokens for request r (0: it rests; negative: it ends, its blocks are free for
+ * this step already and its number for the next), their ids one after the other in tokens. logits (may be NULL):
+ * [n_req][vocab], the row of each request with new tokens is its last one's, other rows are left as they are.
+ * routing_out (may be NULL): [n_layers][new tokens][top_k]. Refused where a request would pass ctx, a step max_tokens,
+ * or the cache its blocks; a step that is refused or fails leaves every request as it was. */
+int rbt_hip_paged_init(rbt_hip *h, int n_req, int ctx, int n_blocks, int block_size, int dtype, int max_tokens);
+int rbt_hip_forward_paged(rbt_hip *h, const int32_t *new_len, const int32_t *tokens, float *logits, int32_t *routing_out);
+
 /* ---- device memory and stream plumbing for hosts without their own HIP code ---- */
 int rbt_hip_malloc(rbt_hip *h, void **dev, uint64_t bytes);
 int rbt_hip_free_dev(rbt_hip *h, void *dev);

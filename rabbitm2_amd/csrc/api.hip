@@ -105,6 +105,24 @@ struct PromptBuf {
     uint8_t *moe = nullptr;  // the MoE block's scratch (scratch_view)
 };
 
+// The whole model on a paged cache (rbt_hip_paged_init): the requests' lengths and the number of free blocks as the
+// last step that succeeded left them, and one allocation of device buffers.
+struct PagedModel {
+    int n_req = 0, ctx = 0, n_blocks = 0, block_size = 0, dtype = 0, max_tokens = 0, max_blocks = 0, n_free = 0;
+    std::vector<int32_t> len;
+    uint8_t *block = nullptr;
+    uint8_t *kc = nullptr, *vc = nullptr;  // [n_layers] caches
+    uint64_t layer_bytes = 0;
+    float *x = nullptr, *xb = nullptr, *q = nullptr, *k = nullptr, *v = nullptr, *ao = nullptr;  // [max_tokens] rows
+    float *last = nullptr, *logits = nullptr;  // [n_req] rows
+    float2 *rope_cs = nullptr;
+    int32_t *in = nullptr;  // a step's input: len, new_len, n_free, the last rows, tokens
+    int32_t *tables = nullptr, *free_list = nullptr, *kv_len = nullptr, *n_free_out = nullptr, *q_start = nullptr,
+            *slots = nullptr, *positions = nullptr, *status = nullptr;
+    int32_t *routing = nullptr;  // [n_layers][max_tokens][top_k]
+    uint8_t *moe = nullptr;      // the MoE block's scratch (scratch_view)
+};
+
 // A tiled copy of one layer's experts (launch_prefill_layout), taken from the blobs at `experts`.
 struct TiledLayer {
     const void *experts = nullptr;
@@ -165,6 +183,7 @@ struct rbt_hip {
     int tok_host_n = 0;
     // this device's scratch array (rbt_hip_moe_dev_noalloc), from hipGetSymbolAddress at init
     void *scratch = nullptr;
+    PagedModel paged;
     void *paged_ws = nullptr;  // the paged attention's workspace (rbt_hip_paged_reserve)
     bool paged_ws_stale = false;  // an attention launch left it without its merge
     // tiled copies of layers' experts for the 128-row grouped GEMMs (rbt_hip_prefill_layout), keyed by
@@ -655,6 +674,8 @@ int model_drop(rbt_hip *h) {
     h->ds = DecodeState{};
     (void)hipFree(h->prompt.block);
     h->prompt = PromptBuf{};
+    (void)hipFree(h->paged.block);
+    h->paged = PagedModel{};
     (void)hipFree(h->rhist);
     h->rhist = nullptr;
     if (h->model) {
@@ -1150,6 +1171,20 @@ int prompt_reserve(rbt_hip *h, int n) {
     return 0;
 }
 
+// RoPE (cos, sin) of every position and pair, with the engine's own expressions in double and the host's libm
+// (rabbit2.c:414-417), so the rotation uses the same floats as the engine.
+std::vector<float2> rope_table(const rbt_config &c, int ctx) {
+    const int half = c.head_dim / 2;
+    std::vector<float2> cs((size_t)ctx * half);
+    for (int p = 0; p < ctx; p++)
+        for (int i = 0; i < half; i++) {
+            const double freq = pow((double)c.rope_theta, -2.0 * i / c.head_dim);
+            const double ang = p * freq;
+            cs[(size_t)p * half + i] = make_float2((float)cos(ang), (float)sin(ang));
+        }
+    return cs;
+}
+
 int prompt_layers(rbt_hip *h, int p0, int T) {
     const rbt_config &c = h->cfg;
     const DecodeState &ds = h->ds;
@@ -1251,6 +1286,7 @@ void rbt_hip_free(rbt_hip *h) {
     (void)hipFree(h->stage);
     if (h->pin) (void)hipHostFree(h->pin);
     (void)hipFree(h->rhist);
+    (void)hipFree(h->paged.block);
     (void)hipFree(h->paged_ws);
     if (h->tok_host) (void)hipHostFree(h->tok_host);
     tiled_drop(h, nullptr, nullptr);
@@ -1708,6 +1744,44 @@ int check_paged_attn(rbt_hip *h, const rbt_paged_kv *kv, const rbt_paged_batch *
     return 1;
 }
 
+// forward() (rabbit2.c:453-542, without the final norm and lm_head) of a planned step's T rows on the paged caches.
+int paged_layers(rbt_hip *h, int T, const int32_t *tokens_dev, bool record) {
+    const rbt_config &c = h->cfg;
+    const PagedModel &p = h->paged;
+    const int D = c.dim, hd = c.head_dim, qd = c.n_heads * hd, kvd = c.n_kv_heads * hd;
+    const Launch L = plain(h);
+    auto vec = [&](uint64_t off) { return reinterpret_cast<const float *>(h->model + off); };
+    const rbt_paged_batch batch{p.n_req, p.max_blocks, p.tables, p.kv_len, p.q_start};
+    HIP_OK(h, launch_prompt_embed(L, c.dtype, h->model + h->tok_emb, D, c.vocab, tokens_dev, T, p.x));
+    for (int l = 0; l < c.n_layers; l++) {
+        const LayerOff &ly = h->layers[(size_t)l];
+        const void *W[3] = {h->model + ly.wq, h->model + ly.wk, h->model + ly.wv};
+        const void *Wo[3] = {h->model + ly.wo, nullptr, nullptr};
+        float *const out[3] = {p.q, p.k, p.v}, *const no_out[3] = {nullptr, nullptr, nullptr};
+        const int rows[3] = {qd, kvd, kvd}, wo_rows[3] = {D, 0, 0};
+        const rbt_paged_kv kv{p.n_blocks, p.block_size, c.n_kv_heads, hd, p.dtype, p.kc + (uint64_t)l * p.layer_bytes,
+                              p.vc + (uint64_t)l * p.layer_bytes, 0};
+        const rbt_paged_rows new_rows{T, c.n_heads, p.q, p.k, p.v, 0, 0, 0, p.q, c.qk_norm ? vec(ly.q_norm) : nullptr,
+                                      c.qk_norm ? vec(ly.k_norm) : nullptr, c.rms_eps,
+                                      reinterpret_cast<const float *>(p.rope_cs), p.ctx, p.positions, p.slots};
+        HIP_OK(h, launch_rmsnorm(L, p.x, vec(ly.attn_norm), D, c.rms_eps, p.xb, T));
+        HIP_OK(h, launch_dense_full(L, c.dtype, p.xb, T, D, W, out, rows, nullptr));
+        if (!rbt_hip_paged_append_dev(h, &kv, &new_rows)) return 0;
+        if (!rbt_hip_paged_attn_dev(h, &kv, &batch, p.q, 0, T, c.n_heads, 0.0f, 0, p.ao, 0)) return 0;
+        HIP_OK(h, launch_dense_full(L, c.dtype, p.ao, T, qd, Wo, no_out, wo_rows, p.x));
+        HIP_OK(h, launch_rmsnorm(L, p.x, vec(ly.ffn_norm), D, c.rms_eps, p.xb, T));
+        rbt_moe_layer ml;
+        if (!rbt_hip_layer(h, l, &ml)) return 0;
+        const MoeForm form = prompt_form(h, &ml, T);
+        Workspace w = scratch_view(p.moe, T, c.n_experts, c.top_k, c.expert_hidden, D, form);
+        if (!moe_block(h, &ml, p.xb, T, p.x, nullptr, nullptr, nullptr, w, form, false)) return 0;
+        if (record)
+            HIP_OK(h, hipMemcpyAsync(p.routing + (size_t)l * T * c.top_k, w.routing, 4 * (size_t)T * c.top_k,
+                                     hipMemcpyDeviceToDevice, h->stream));
+    }
+    return 1;
+}
+
 // The attention's workspace: one size for every call, so that it never moves under a captured graph.
 int paged_ws_reserve(rbt_hip *h) {
     if (h->paged_ws) return 1;
@@ -1779,6 +1853,172 @@ int rbt_hip_paged_attn_dev(rbt_hip *h, const rbt_paged_kv *kv, const rbt_paged_b
 int rbt_hip_paged_reserve(rbt_hip *h) {
     if (!h) return fail(nullptr, "paged_reserve: handle is NULL");
     return set_device(h) && paged_ws_reserve(h);
+}
+
+int rbt_hip_paged_init(rbt_hip *h, int n_req, int ctx, int n_blocks, int block_size, int dtype, int max_tokens) {
+    if (!h) return fail(nullptr, "paged_init: handle is NULL");
+    if (!h->model) return fail(h, "paged_init: no model");
+    const rbt_config &c = h->cfg;
+    if (ctx < 0) return fail(h, "paged_init: negative context");
+    if (ctx == 0) ctx = c.max_seq < 512 ? c.max_seq : 512;  // rabbit2.c:684
+    if (ctx > c.max_seq) ctx = c.max_seq;                   // rabbit2.c:685
+    if (n_req < 1 || n_req > kPagedMaxReq) return fail(h, "paged_init: n_req %d outside [1, %d]", n_req, kPagedMaxReq);
+    if (max_tokens < 1 || max_tokens > 65535) return fail(h, "paged_init: max_tokens %d outside [1, 65535]", max_tokens);
+    if (dtype != RBT_DT_F32 && dtype != RBT_DT_BF16) return fail(h, "paged_init: invalid dtype %d", dtype);
+    if (n_blocks < 1 || block_size < 1 || (int64_t)n_blocks * block_size > INT32_MAX)
+        return fail(h, "paged_init: %d blocks of %d positions", n_blocks, block_size);
+    const int qd = c.n_heads * c.head_dim, kvd = c.n_kv_heads * c.head_dim;
+    if (c.head_dim > kPagedMaxHd || !dense_full_supported(c.dtype, max_tokens, c.dim, std::max(std::max(qd, kvd), c.vocab), nullptr) ||
+        !dense_full_supported(c.dtype, max_tokens, qd, c.dim, nullptr))
+        return fail(h, "paged_init: dims %d and %d (%d heads of %d) are not multiples of 4, or too large", c.dim, qd, c.n_heads,
+                    c.head_dim);
+    if (!set_device(h) || !paged_ws_reserve(h)) return 0;
+    HIP_OK(h, hipStreamSynchronize(h->stream));
+    (void)hipFree(h->paged.block);
+    h->paged = PagedModel{};
+    PagedModel p;
+    p.n_req = n_req;
+    p.ctx = ctx;
+    p.n_blocks = p.n_free = n_blocks;
+    p.block_size = block_size;
+    p.dtype = dtype;
+    p.max_tokens = max_tokens;
+    p.max_blocks = ctx / block_size + (ctx % block_size != 0);
+    p.len.assign((size_t)n_req, 0);
+    p.layer_bytes = align_up((uint64_t)n_blocks * block_size * kvd * (dtype == RBT_DT_BF16 ? 2 : 4), 256);
+    const uint64_t T = (uint64_t)max_tokens, R = (uint64_t)n_req, rows = std::min(T, R);
+    uint64_t off = 0;
+    auto carve = [&](uint64_t bytes) {
+        const uint64_t at = off;
+        off = align_up(off + bytes, 256);
+        return at;
+    };
+    const uint64_t o_kc = carve(p.layer_bytes * c.n_layers), o_vc = carve(p.layer_bytes * c.n_layers);
+    const uint64_t o_x = carve(4 * T * c.dim), o_xb = carve(4 * T * c.dim), o_q = carve(4 * T * qd), o_k = carve(4 * T * kvd),
+                   o_v = carve(4 * T * kvd), o_ao = carve(4 * T * qd);
+    const uint64_t o_last = carve(4 * rows * c.dim), o_lg = carve(4 * rows * c.vocab);
+    const uint64_t o_rope = carve(8 * (uint64_t)ctx * (c.head_dim / 2)), o_in = carve(4 * (3 * R + 1 + T));
+    const uint64_t o_t = carve(4 * R * p.max_blocks), o_free = carve(4 * (uint64_t)n_blocks), o_kv = carve(4 * R),
+                   o_fo = carve(4), o_qs = carve(4 * (R + 1)), o_sl = carve(4 * T), o_po = carve(4 * T), o_st = carve(4);
+    const uint64_t o_rt = carve(4 * T * c.n_layers * c.top_k);
+    const uint64_t o_moe = carve(std::max(moe_scratch_bytes(max_tokens, c.n_experts, c.top_k, c.expert_hidden, c.dim, kMoeGroupedFull),
+                                          moe_scratch_bytes(max_tokens, c.n_experts, c.top_k, c.expert_hidden, c.dim, kMoeGeneral)));
+    HIP_OK(h, hipMalloc(&p.block, off));
+    auto f32 = [&](uint64_t at) { return reinterpret_cast<float *>(p.block + at); };
+    auto i32 = [&](uint64_t at) { return reinterpret_cast<int32_t *>(p.block + at); };
+    p.kc = p.block + o_kc;
+    p.vc = p.block + o_vc;
+    p.x = f32(o_x);
+    p.xb = f32(o_xb);
+    p.q = f32(o_q);
+    p.k = f32(o_k);
+    p.v = f32(o_v);
+    p.ao = f32(o_ao);
+    p.last = f32(o_last);
+    p.logits = f32(o_lg);
+    p.rope_cs = reinterpret_cast<float2 *>(p.block + o_rope);
+    p.in = i32(o_in);
+    p.tables = i32(o_t);
+    p.free_list = i32(o_free);
+    p.kv_len = i32(o_kv);
+    p.n_free_out = i32(o_fo);
+    p.q_start = i32(o_qs);
+    p.slots = i32(o_sl);
+    p.positions = i32(o_po);
+    p.status = i32(o_st);
+    p.routing = i32(o_rt);
+    p.moe = p.block + o_moe;
+    const std::vector<float2> cs = rope_table(c, ctx);
+    std::vector<int32_t> ids((size_t)n_blocks);
+    for (int i = 0; i < n_blocks; i++) ids[(size_t)i] = n_blocks - 1 - i;  // block 0 is on top
+    hipError_t e = HIP_TRY(hipMemcpy(p.rope_cs, cs.data(), cs.size() * sizeof(float2), hipMemcpyHostToDevice));
+    if (e == hipSuccess) e = HIP_TRY(hipMemcpy(p.free_list, ids.data(), 4 * ids.size(), hipMemcpyHostToDevice));
+    if (e != hipSuccess) {
+        (void)hipFree(p.block);
+        return fail(h, "paged_init: %s failed: %s", failed_call(), hipGetErrorString(e));
+    }
+    h->paged = p;
+    return 1;
+}
+
+int rbt_hip_forward_paged(rbt_hip *h, const int32_t *new_len, const int32_t *tokens, float *logits, int32_t *routing_out) {
+    if (!h) return fail(nullptr, "forward_paged: handle is NULL");
+    PagedModel &p = h->paged;
+    if (!p.block) return fail(h, "forward_paged: no paged state (rbt_hip_paged_init)");
+    if (!new_len) return fail(h, "forward_paged: NULL argument");
+    const rbt_config &c = h->cfg;
+    std::vector<int32_t> len(p.len), last;
+    int64_t T = 0, freed = 0, need = 0;
+    auto pages = [&](int64_t n) { return (n + p.block_size - 1) / p.block_size; };
+    for (int r = 0; r < p.n_req; r++) {
+        if (new_len[r] < 0) {
+            freed += pages(len[(size_t)r]);
+            len[(size_t)r] = 0;
+            continue;
+        }
+        const int64_t n = (int64_t)len[(size_t)r] + new_len[r];
+        if (n > p.ctx)
+            return fail(h, "forward_paged: request %d: %d positions and %d more in a context of %d", r, len[(size_t)r],
+                        new_len[r], p.ctx);
+        need += pages(n) - pages(len[(size_t)r]);
+        len[(size_t)r] = (int32_t)n;
+        T += new_len[r];
+        if (new_len[r] > 0) last.push_back((int32_t)std::min<int64_t>(T - 1, INT32_MAX));
+    }
+    if (T > p.max_tokens) return fail(h, "forward_paged: %lld tokens, room for %d", (long long)T, p.max_tokens);
+    if (need > p.n_free + freed)
+        return fail(h, "forward_paged: %lld blocks are lacking", (long long)(need - p.n_free - freed));
+    if (T > 0 && !tokens) return fail(h, "forward_paged: NULL argument");
+    for (int64_t t = 0; t < T; t++)
+        if (tokens[t] < 0 || tokens[t] >= c.vocab) return fail(h, "token %d out of range", tokens[t]);
+    if (!set_device(h)) return 0;
+    // The plan reads the lengths and the free count of the last step that succeeded, so that a step that fails can be
+    // run again: it takes the same blocks from the same stack.
+    const size_t R = (size_t)p.n_req;
+    std::vector<int32_t> in(3 * R + 1 + (size_t)T, 0);
+    std::copy(p.len.begin(), p.len.end(), in.begin());
+    std::copy(new_len, new_len + R, in.begin() + (ptrdiff_t)R);
+    in[2 * R] = p.n_free;
+    std::copy(last.begin(), last.end(), in.begin() + (ptrdiff_t)(2 * R + 1));
+    if (T > 0) std::copy(tokens, tokens + T, in.begin() + (ptrdiff_t)(3 * R + 1));
+    HIP_OK(h, hipMemcpyAsync(p.in, in.data(), 4 * in.size(), hipMemcpyHostToDevice, h->stream));
+    const int32_t *last_dev = p.in + 2 * R + 1, *tokens_dev = p.in + 3 * R + 1;
+    const rbt_paged_plan plan{p.n_req, p.max_blocks, p.n_blocks, p.block_size, (int)T, p.in, p.in + R, p.tables, p.free_list,
+                              p.in + 2 * R, p.kv_len, p.n_free_out, p.q_start, p.slots, p.positions, p.status};
+    if (!rbt_hip_paged_plan_dev(h, &plan)) return 0;
+    if (T > 0) {
+        const GroupedCall user_call = h->grouped;  // as in prompt_block
+        const int ok = paged_layers(h, (int)T, tokens_dev, routing_out != nullptr);
+        h->grouped = user_call;
+        if (!ok) return 0;
+    }
+    const int n = (int)last.size();
+    if (logits && n > 0) {
+        Launch L = plain(h);
+        const void *W[3] = {h->model + h->lm_head, nullptr, nullptr};
+        float *const out[3] = {p.logits, nullptr, nullptr};
+        const int rows[3] = {c.vocab, 0, 0};
+        HIP_OK(h, launch_gather_rows(L, p.x, last_dev, n, c.dim, p.last));
+        HIP_OK(h, launch_rmsnorm(L, p.last, reinterpret_cast<const float *>(h->model + h->final_norm), c.dim, c.rms_eps, p.xb, n));
+        HIP_OK(h, launch_dense_full(L, c.dtype, p.xb, n, c.dim, W, out, rows, nullptr));
+        for (int r = 0, i = 0; r < p.n_req;) {  // runs of requests that have new tokens
+            int m = 0;
+            while (r + m < p.n_req && new_len[r + m] > 0) m++;
+            if (m > 0)
+                HIP_OK(h, hipMemcpyAsync(logits + (size_t)r * c.vocab, p.logits + (size_t)i * c.vocab,
+                                         4 * (size_t)m * c.vocab, hipMemcpyDeviceToHost, h->stream));
+            i += m;
+            r += m + 1;
+        }
+    }
+    if (routing_out && T > 0)
+        HIP_OK(h, hipMemcpyAsync(routing_out, p.routing, 4 * (size_t)c.n_layers * (size_t)T * c.top_k, hipMemcpyDeviceToHost,
+                                 h->stream));
+    HIP_OK(h, hipStreamSynchronize(h->stream));
+    p.len = len;
+    p.n_free += (int)(freed - need);
+    h->cache_hits += (uint64_t)c.n_layers * (uint64_t)T * c.top_k;
+    return prof_harvest(h);
 }
 
 int rbt_hip_malloc(rbt_hip *h, void **dev, uint64_t bytes) {
@@ -2008,17 +2248,8 @@ int rbt_hip_batch_init(rbt_hip *h, int n_seq, int ctx) {
     ds.seq = reinterpret_cast<int32_t *>(b + o_seq);
     ds.st = reinterpret_cast<StepState *>(b + o_st);
     HIP_OK(h, hipMemset(ds.block, 0, off));
-    // RoPE (cos, sin) of every position and pair, with the engine's own expressions in double and the
-    // host's libm (rabbit2.c:414-417), so the rotation uses the same floats as the engine
     {
-        const int half = c.head_dim / 2;
-        std::vector<float2> cs((size_t)ctx * half);
-        for (int p = 0; p < ctx; p++)
-            for (int i = 0; i < half; i++) {
-                const double freq = pow((double)c.rope_theta, -2.0 * i / c.head_dim);
-                const double ang = p * freq;
-                cs[(size_t)p * half + i] = make_float2((float)cos(ang), (float)sin(ang));
-            }
+        const std::vector<float2> cs = rope_table(c, ctx);
         const hipError_t e = hipMemcpy(ds.rope_cs, cs.data(), cs.size() * sizeof(float2), hipMemcpyHostToDevice);
         if (e != hipSuccess) {
             (void)hipFree(ds.block);

@@ -1718,6 +1718,12 @@ __global__ void attn_clear_kernel(uint8_t *ws) {
         AttnWs<false>::header(ws)->taken[threadIdx.x][0] = AttnWs<true>::header(ws)->taken[threadIdx.x][0] = 0;
 }
 
+// Rows ids[i] of x in turn: the last new token of each request, for its logits. A block to a row.
+__global__ __launch_bounds__(256) void gather_rows_kernel(const float *x, const int32_t *ids, int D, float *out) {
+    const float *src = x + (size_t)ids[blockIdx.x] * D;
+    for (int i = threadIdx.x; i < D; i += 256) out[(size_t)blockIdx.x * D + i] = src[i];
+}
+
 PagedDims dims_of(const rbt_paged_kv &kv) {
     PagedDims d;
     d.n_blocks = kv.n_blocks;
@@ -1891,6 +1897,10 @@ hipError_t launch_paged_attn(const Launch &L, const PagedAttn &p) {
 }
 
 hipError_t launch_paged_merge(const Launch &L, const PagedAttn &p) { return launch_tiled(L, p, true); }
+
+hipError_t launch_gather_rows(const Launch &L, const float *x, const int32_t *ids, int n, int D, float *out) {
+    return launch(L, gather_rows_kernel, dim3((unsigned)n), dim3(256), 0, x, ids, D, out);
+}
 
 hipError_t launch_paged_clear(const Launch &L, void *ws) {
     return launch(L, attn_clear_kernel, dim3(1), dim3(64), 0, static_cast<uint8_t *>(ws));

@@ -433,6 +433,8 @@ struct PagedAttn {
 bool paged_attn_tiled(const PagedAttn &p);
 hipError_t launch_paged_attn(const Launch &L, const PagedAttn &p);
 hipError_t launch_paged_merge(const Launch &L, const PagedAttn &p);
+// out [n][D] = x[ids[i]]
+hipError_t launch_gather_rows(const Launch &L, const float *x, const int32_t *ids, int n, int D, float *out);
 hipError_t launch_paged_clear(const Launch &L, void *ws);
 
 // Dense matvec (one row per wave).

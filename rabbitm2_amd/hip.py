@@ -26,7 +26,7 @@ EXPORTS = (
     "rbt_hip_generate_stream", "rbt_hip_routing_history", "rbt_hip_expert_cache_replay",
     "rbt_hip_moe_dev_noalloc", "rbt_hip_prefill_layout", "rbt_hip_prefill_layout_drop", "rbt_hip_profiler_attached",
     "rbt_hip_tile_rows", "rbt_hip_paged_plan_dev", "rbt_hip_paged_append_dev", "rbt_hip_paged_attn_dev",
-    "rbt_hip_paged_reserve",
+    "rbt_hip_paged_reserve", "rbt_hip_paged_init", "rbt_hip_forward_paged",
 )
 
 TOKEN_FN = C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_int32)
@@ -136,6 +136,8 @@ def lib():
         L.rbt_hip_paged_attn_dev.argtypes = [vp, C.POINTER(PagedKV), C.POINTER(PagedBatch), vp, u64, i32, i32, f32, i32,
                                              vp, u64]
         L.rbt_hip_paged_reserve.argtypes = [vp]
+        L.rbt_hip_paged_init.argtypes = [vp, i32, i32, i32, i32, i32, i32]
+        L.rbt_hip_forward_paged.argtypes = [vp, vp, vp, vp, vp]
         _lib = L
     return _lib
 
@@ -421,6 +423,19 @@ class Device:
 
     def paged_reserve(self):
         self._check(self.L.rbt_hip_paged_reserve(self.h))
+
+    def paged_init(self, n_req, ctx, n_blocks, block_size, dtype, max_tokens):
+        self._check(self.L.rbt_hip_paged_init(self.h, n_req, ctx, n_blocks, block_size, dtype, max_tokens))
+
+    def forward_paged(self, new_len, tokens, vocab, n_layers, top_k):
+        """One step of all requests: (logits [n_req][vocab], 0 where a request has no new tokens; routing
+        [n_layers][new tokens][top_k])."""
+        new_len = np.ascontiguousarray(new_len, dtype=np.int32)
+        tokens = np.ascontiguousarray(tokens, dtype=np.int32)
+        logits = np.zeros((new_len.size, vocab), np.float32)
+        routing = np.zeros((n_layers, tokens.size, top_k), np.int32)
+        self._check(self.L.rbt_hip_forward_paged(self.h, _p(new_len), _p(tokens), _p(logits), _p(routing)))
+        return logits, routing
 
 
 def profiler_attached():

@@ -59,6 +59,8 @@ def test_good_arguments_reach_the_handle_check():
     for ok in (attn(), append(), do_plan(plan())):
         assert ok == 0 and "handle is NULL" in message()
     assert hip.lib().rbt_hip_paged_reserve(None) == 0 and "handle is NULL" in message()
+    assert hip.lib().rbt_hip_paged_init(None, 1, 0, 1, 1, 0, 1) == 0 and "handle is NULL" in message()
+    assert hip.lib().rbt_hip_forward_paged(None, None, None, None, None) == 0 and "handle is NULL" in message()
 
 
 BAD_KV = [dict(n_blocks=0), dict(block_size=0), dict(n_kv_heads=0), dict(head_dim=0), dict(head_dim=257),
