@@ -1860,7 +1860,10 @@ template <int DT, int HDP>
 hipError_t launch_attn(const Launch &L, AttnArgs a, bool merge) {
     using Sh = AttnShape<DT, HDP>;
     const int lds = attn_blocks<DT, HDP>(a);
-    if (merge) return launch(L, attn_merge_kernel<HDP>, dim3(1024), dim3(256), 0, a);
+    if (merge) {  // no more blocks than the rows need, and two rounds of them (prompt of 4096: 208 us against 213 with 1024)
+        const int64_t n = (int64_t)a.T * a.n_heads / (256 / HDP) + 1;
+        return launch(L, attn_merge_kernel<HDP>, dim3((unsigned)(n < 4096 ? n : 4096)), dim3(256), 0, a);
+    }
     static std::atomic<uint64_t> asked{0};
     const hipError_t e = ask_lds(attn_kernel<DT, HDP>, kLdsBytes, asked);
     if (e != hipSuccess) return e;
