@@ -817,9 +817,12 @@ struct WaveState {
 // 32 positions, staged from byte k_off (keys) and v_off (values) of LDS on, parts `part` bytes apart; between(i) is
 // called among the products, for i = 0 .. HDP / 16 NP - 1 in turn; seen(n): bit 4 t + i, whether query n of this lane
 // sees key 16 t + 4 g + i of them (asked where !full).
-template <int HDP, int NQ, int QP, int NP, int part, typename Tile, typename Between, typename Seen>
+// Mid: a call between the keys' last use and the values' first (and no value is read before it), or NoMid.
+struct NoMid {};
+template <int HDP, int NQ, int QP, int NP, int part, typename Tile, typename Between, typename Seen, typename Mid>
 __device__ __forceinline__ void attn_step(WaveState<HDP, NQ, QP> &w, const Tile &tile, int k_off, int v_off, bool full,
-                                          Between between, Seen seen) {
+                                          Between between, Seen seen, Mid mid) {
+    constexpr bool kMid = !std::is_same_v<Mid, NoMid>;
     // Consecutive products go to different sums: a sum's next product waits for its last. The operands of the next
     // products are read from LDS before those of the last ones are used.
     constexpr int KI = HDP / 32 * NP, VI = HDP / 32 * NP;  // (k-step, part) and (pair of 16 dims, part)
@@ -849,7 +852,7 @@ __device__ __forceinline__ void attn_step(WaveState<HDP, NQ, QP> &w, const Tile 
     for (int i = 0; i < KI; ++i) {
         if (i + 1 < KI)
             read_k(i + 1, k[(i + 1) & 1]);
-        else
+        else if (!kMid)
             read_v(0, v[0]);
         u32x4 q3[NQ];
         if (QP < 3 && i % NP == 0)
@@ -914,6 +917,10 @@ __device__ __forceinline__ void attn_step(WaveState<HDP, NQ, QP> &w, const Tile 
                 w.l[n] += e[4 * t + i];
             }
         split3(e, p[n], w.pc);
+    }
+    if constexpr (kMid) {
+        mid();
+        read_v(0, v[0]);
     }
 #pragma unroll
     for (int i = 0; i < VI; ++i) {
@@ -1037,6 +1044,7 @@ struct Stage {
     u32x4 k[N][LD], v[N][LD];
     PartConsts pc;
 
+    template <bool K, bool V>
     __device__ __forceinline__ void load(const AttnArgs &a, const uint64_t *s_tab, int page0, int kvh, int j, int last,
                                          int tid) {
         const int row = tid / CH, chunk = min(tid % CH, a.d.hd / 8 - 1);  // behind the head's end: its last chunk
@@ -1047,8 +1055,8 @@ struct Stage {
             const uint64_t at = row_at<DT>(a, s_tab, page0, head_off, min(j + row + i * ROWS, last)) + 8 * chunk * esz;
 #pragma unroll
             for (int x = 0; x < LD; ++x) {
-                k[i][x] = ld_kv<ONCE>(static_cast<const uint8_t *>(a.kc) + at + 16 * x);
-                v[i][x] = ld_kv<ONCE>(static_cast<const uint8_t *>(a.vc) + at + 16 * x);
+                if (K) k[i][x] = ld_kv<ONCE>(static_cast<const uint8_t *>(a.kc) + at + 16 * x);
+                if (V) v[i][x] = ld_kv<ONCE>(static_cast<const uint8_t *>(a.vc) + at + 16 * x);
             }
         }
     }
@@ -1065,14 +1073,10 @@ struct Stage {
             for (int y = 0; y < 3; ++y) *reinterpret_cast<u32x4 *>(smem + off + y * part) = p[y];
         }
     }
-    __device__ __forceinline__ void store(int k_off, int v_off, int part, int tid) {
-        const int at = tid / CH * PaddedTile<HDP>::ROW + 16 * (tid % CH);
+    __device__ __forceinline__ void store(const u32x4 (&r)[N][LD], int to, int part, int tid) {
+        const int at = to + tid / CH * PaddedTile<HDP>::ROW + 16 * (tid % CH);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int off = at + i * ROWS * PaddedTile<HDP>::ROW;
-            put(k[i], k_off + off, part);
-            put(v[i], v_off + off, part);
-        }
+        for (int i = 0; i < N; ++i) put(r[i], at + i * ROWS * PaddedTile<HDP>::ROW, part);
     }
 };
 
@@ -1385,14 +1389,16 @@ __device__ __forceinline__ void attn_thin(const AttnArgs &a, int block, int bloc
             stretches([&](int w0, int w1, int page0, bool bad) {
                 Stage<DT, HDP, 32, 64, true> st;
                 int j = w0 + 32 * wv;
-                if (j < w1) st.load(a, s_tab, page0, x.kvh, j, w1 - 1, lane);
+                if (j < w1) st.template load<true, true>(a, s_tab, page0, x.kvh, j, w1 - 1, lane);
                 for (; j < w1; j += 128) {
                     __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
-                    st.store(at, v_off, 0, lane);
+                    st.store(st.k, at, 0, lane);
+                    st.store(st.v, v_off, 0, lane);
                     __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
-                    if (j + 128 < w1) st.load(a, s_tab, page0, x.kvh, j + 128, w1 - 1, lane);
+                    if (j + 128 < w1) st.template load<true, true>(a, s_tab, page0, x.kvh, j + 128, w1 - 1, lane);
                     attn_step<HDP, 1, 3, 1, 0>(w, tl, at, v_off, whole(j, 32, w1, bad), [](int) {},
-                                               [&](int n) { return seen_bits(a, j, w1, w.pos[n], s_tab, page0, bad); });
+                                               [&](int n) { return seen_bits(a, j, w1, w.pos[n], s_tab, page0, bad); },
+                                               NoMid());
                 }
             });
             w.l[0] = group_sum(w.l[0]);
@@ -1482,12 +1488,14 @@ __device__ __forceinline__ void attn_thin(const AttnArgs &a, int block, int bloc
 template <int DT, int HDP>
 struct WideShape {
     static constexpr int NP = DT == RBT_DT_BF16 ? 1 : 3;
-    // bf16: two buffers that direct copies fill in turn; f32: one of parts, through registers
+    // bf16: two buffers of keys and values that direct copies fill in turn; f32: one of parts, through registers, of
+    // the keys and then of the values, which leaves room for the query rows' third part (prompt of 4096 tokens, 16 heads
+    // of 128: 414 us; both at once, the queries in registers, 78 of them spilled: 436; heads of 64: 134 against 130)
     static constexpr bool COPY = DT == RBT_DT_BF16;
     using Tile = std::conditional_t<COPY, SwizzledTile<HDP>, PaddedTile<HDP>>;
-    static constexpr int PART = 32 * Tile::ROW, BUF = 2 * NP * PART;
-    // with two blocks to a CU there are registers for two of the query rows' three parts
-    static constexpr int QP = COPY && HDP == 128 ? 2 : 3, Q_AT = COPY ? 2 * BUF : BUF;
+    static constexpr int PART = 32 * Tile::ROW, BUF = (COPY ? 2 : 1) * NP * PART;
+    // there are registers for two of the query rows' three parts; the third in LDS, where it fits
+    static constexpr int QP = HDP == 128 || (!COPY && HDP == 256) ? 2 : 3, Q_AT = COPY ? 2 * BUF : BUF;
     static constexpr int TILE = Q_AT + (QP < 3 ? kWideRows * PaddedTile<HDP>::ROW : 0);
     static constexpr int PER_CU = HDP <= 128 ? 2 : 1;
     static_assert(sizeof(RowShared) <= (size_t)TILE, "row_any's LDS");
@@ -1522,12 +1530,12 @@ __device__ __forceinline__ void attn_wide(const AttnArgs &a, int block, int bloc
             if (w0 != x.k0) tab.ask(a, x.r, w0, w1);
             const bool bad = tab.fill(a, s_tab);
             // the wave's part of 32 staged positions from j on: whether it has any
-            auto step = [&](int j, int off, auto between) {
+            auto step = [&](int j, int off, auto between, auto mid) {
                 if (!active || j >= w1 || j > wb || (a.window > 0 && j + 31 <= wa - a.window)) return false;
                 const bool full = !bad && j + 32 <= min(w1, wa + 1) && (a.window <= 0 || j > wb - a.window);
                 attn_step<HDP, 2, Sh::QP, Sh::NP, Sh::PART>(
-                    w, tl, off, off + Sh::NP * Sh::PART, full, between,
-                    [&](int n) { return seen_bits(a, j, w1, w.pos[n], s_tab, page0, bad); });
+                    w, tl, off, Sh::COPY ? off + Sh::PART : off, full, between,
+                    [&](int n) { return seen_bits(a, j, w1, w.pos[n], s_tab, page0, bad); }, mid);
                 return true;
             };
             if constexpr (Sh::COPY) {
@@ -1549,7 +1557,7 @@ __device__ __forceinline__ void attn_wide(const AttnArgs &a, int block, int bloc
                     const bool done = step(j, buf, [&](int i) {
                         if (i == 0) look(j + 64);
                         if (i == 2) cp.aim();
-                    });
+                    }, NoMid());
                     if (!done) {
                         look(j + 64);
                         cp.aim();
@@ -1558,13 +1566,19 @@ __device__ __forceinline__ void attn_wide(const AttnArgs &a, int block, int bloc
                 }
             } else {
                 Stage<DT, HDP, 32, 256, false> st;
-                st.load(a, s_tab, page0, x.kvh, w0, w1 - 1, tid);
+                st.template load<true, false>(a, s_tab, page0, x.kvh, w0, w1 - 1, tid);
                 for (int jt = w0; jt < w1; jt += 32) {
                     __syncthreads();
-                    st.store(0, Sh::NP * Sh::PART, Sh::PART, tid);
+                    st.store(st.k, 0, Sh::PART, tid);
+                    st.template load<false, true>(a, s_tab, page0, x.kvh, jt, w1 - 1, tid);
                     __syncthreads();
-                    if (jt + 32 < w1) st.load(a, s_tab, page0, x.kvh, jt + 32, w1 - 1, tid);
-                    step(jt, 0, [](int) {});
+                    auto values = [&]() {
+                        __syncthreads();  // the keys have been read
+                        st.store(st.v, 0, Sh::PART, tid);
+                        if (jt + 32 < w1) st.template load<true, false>(a, s_tab, page0, x.kvh, jt + 32, w1 - 1, tid);
+                        __syncthreads();
+                    };
+                    if (!step(jt, 0, [](int) {}, values)) values();
                 }
             }
         }
