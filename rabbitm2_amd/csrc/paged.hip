@@ -498,10 +498,11 @@ __global__ __launch_bounds__(256) void attn_any_kernel(AttnArgs a) {
 // and its state are f32. Outputs are as far from 64 bits as f32 arithmetic leaves them (3e-7 of their size; two parts
 // would be a third faster and 16 bits).
 //
-// What bounds it: a prompt of 4096 tokens (16 heads of 128, bf16) takes 216 us, three products of 69 GFLOP: 955 TFLOP/s
-// of the matrix cores in all, where a large library product reaches 1166; the attention launch alone runs at 1070, the
-// rest joins pieces. 64 decoding sequences of up to 8192 positions take 216 us, 5.8 TB/s of cache. Small steps are
-// latency: the schedule, pages, queries and first keys one after the other, and two launches (one sequence: 16 us).
+// What bounds it: a prompt of 4096 tokens (16 heads of 128, bf16) takes 208 us, 206 GFLOP in its three products: 990
+// TFLOP/s, where a large library product reaches 1200; the matrix units are busy 75% of the inner loop, items' starts
+// and ends and the joining of pieces take 20 us each. 64 decoding sequences of up to 8192 positions take 216 us, 5.8
+// TB/s of cache. Small steps are latency: the schedule, pages, queries and first keys one after the other, and two
+// launches (one sequence: 16 us).
 //
 // Not finite: a position that a row does not see has weight 0, but 0 times an infinity is NaN, so rows whose
 // result is not finite are computed again by row_any, which reads seen positions only. Rows past the positions
