@@ -1868,10 +1868,14 @@ int rbt_hip_paged_init(rbt_hip *h, int n_req, int ctx, int n_blocks, int block_s
     if (n_blocks < 1 || block_size < 1 || (int64_t)n_blocks * block_size > INT32_MAX)
         return fail(h, "paged_init: %d blocks of %d positions", n_blocks, block_size);
     const int qd = c.n_heads * c.head_dim, kvd = c.n_kv_heads * c.head_dim;
-    if (c.head_dim > kPagedMaxHd || !dense_full_supported(c.dtype, max_tokens, c.dim, std::max(std::max(qd, kvd), c.vocab), nullptr) ||
+    const int esz = dtype == RBT_DT_BF16 ? 2 : 4, max_blocks = ctx / block_size + (ctx % block_size != 0);
+    if ((int64_t)max_blocks * block_size > kPagedMaxLen || (double)n_blocks * block_size * kvd * esz * c.n_layers > 1e15)
+        return fail(h, "paged_init: %d blocks of %d positions for contexts of %d", n_blocks, block_size, ctx);
+    if (c.head_dim > kPagedMaxHd || std::max(qd, kvd) > (1 << 20) || (int64_t)max_tokens * c.n_heads > INT32_MAX ||
+        !dense_full_supported(c.dtype, max_tokens, c.dim, std::max(std::max(qd, kvd), c.vocab), nullptr) ||
         !dense_full_supported(c.dtype, max_tokens, qd, c.dim, nullptr))
-        return fail(h, "paged_init: dims %d and %d (%d heads of %d) are not multiples of 4, or too large", c.dim, qd, c.n_heads,
-                    c.head_dim);
+        return fail(h, "paged_init: dims %d and %d (%d heads of %d, %d tokens) are not multiples of 4, or too large", c.dim, qd,
+                    c.n_heads, c.head_dim, max_tokens);
     if (!set_device(h) || !paged_ws_reserve(h)) return 0;
     HIP_OK(h, hipStreamSynchronize(h->stream));
     (void)hipFree(h->paged.block);
@@ -1883,9 +1887,9 @@ int rbt_hip_paged_init(rbt_hip *h, int n_req, int ctx, int n_blocks, int block_s
     p.block_size = block_size;
     p.dtype = dtype;
     p.max_tokens = max_tokens;
-    p.max_blocks = ctx / block_size + (ctx % block_size != 0);
+    p.max_blocks = max_blocks;
     p.len.assign((size_t)n_req, 0);
-    p.layer_bytes = align_up((uint64_t)n_blocks * block_size * kvd * (dtype == RBT_DT_BF16 ? 2 : 4), 256);
+    p.layer_bytes = align_up((uint64_t)n_blocks * block_size * kvd * esz, 256);
     const uint64_t T = (uint64_t)max_tokens, R = (uint64_t)n_req, rows = std::min(T, R);
     uint64_t off = 0;
     auto carve = [&](uint64_t bytes) {

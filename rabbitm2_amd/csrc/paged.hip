@@ -496,7 +496,7 @@ __global__ __launch_bounds__(256) void attn_any_kernel(AttnArgs a) {
 // Precision: bf16 keys and values enter exactly. f32 operands are cut into three bf16 parts of 8 bits each (exact: 24
 // bits), and the products of parts down to 2^-24 are taken: three for a bf16 cache, six for an f32 one. Sums, the softmax
 // and its state are f32. Outputs are as far from 64 bits as f32 arithmetic leaves them (3e-7 of their size; two parts
-// would be a third faster and 16 bits).
+// would leave 16 bits and save a third of the products).
 //
 // What bounds it: a prompt of 4096 tokens (16 heads of 128, bf16) takes 208 us, 206 GFLOP in its three products: 990
 // TFLOP/s, where a large library product reaches 1200; the matrix units are busy 75% of the inner loop, items' starts
@@ -507,11 +507,7 @@ __global__ __launch_bounds__(256) void attn_any_kernel(AttnArgs a) {
 // Not finite: a position that a row does not see has weight 0, but 0 times an infinity is NaN, so rows whose
 // result is not finite are computed again by row_any, which reads seen positions only. Rows past the positions
 // repeat the last one's, with weight 0.
-constexpr int kWideRows = 128, kThinRows = 16;
 constexpr int kTabPages = 512;  // pages whose places are held in LDS at a time
-constexpr int kMaxChunk = kPagedMaxLen;  // positions, a multiple of 128
-static_assert(kMaxChunk % 128 == 0, "whole tiles");
-
 // Workspace: for the wide and the thin blocks each a header (chunk length, blocks of the merge) and the prefix sums of
 // those and of the partial units over the requests, then their partials: units of 16 rows, m [16], l [16],
 // o [16][HDP].
@@ -530,94 +526,11 @@ struct AttnWs {
     static constexpr int max_units(int hdp) { return (int)((kBytes - sizeof(AttnHeader)) / 4 / unit_floats(hdp)); }
 };
 
-// How a request's rows are cut: nt tiles of tr rows, and each tile's positions into pieces of at most `chunk`. Tile t
-// spans up to S(t) = min(p0 + ceil((t + 1) tr / G), limit) positions, which grow with t, so that tiles from T(c) =
-// floor((c chunk - p0) G / tr) on have more than c pieces. The first c0 pieces are every tile's (T = 0), nc is the
-// last tile's number, and the tiles before t have pieces_before(t) = sum over c of max(0, t - T(c)) in all.
-// rows 0: not of this kind.
-template <bool THIN>
-constexpr int kTileRows = THIN ? kThinRows : kWideRows;
-struct Cut {
-    int rows, nt, nc, c0, p0, limit, chunk, G;
-};
 template <bool THIN>
 __device__ __forceinline__ Cut cut_of(const AttnArgs &a, const Request &q, int chunk) {
-    Cut c;
-    constexpr int tr = kTileRows<THIN>;
-    c.G = (int)a.group.d;
-    c.rows = q.m * c.G;
-    if (THIN != (a.thin && c.rows <= kThinRows)) c.rows = 0;
-    c.nt = (c.rows + tr - 1) / tr;
-    c.p0 = q.p0;
-    // all positions up to a tile's last row, or a window's and what its tokens span
-    c.limit = a.window > 0 ? min(q.n, min(a.window, q.n) + (tr - 1) / c.G + 1) : q.n;
-    c.chunk = chunk;
-    c.nc = max(1, (int)(((uint32_t)c.limit + (uint32_t)(chunk - 1)) / (uint32_t)chunk));
-    c.c0 = q.p0 > 0 ? min(c.nc, q.p0 / chunk + 1) : 1;
-    return c;
-}
-template <bool THIN>
-__device__ __forceinline__ int first_with(const Cut &c, int piece) {  // T(piece), for piece < nc; below 0 before c0
-    return (int)(((long long)piece * c.chunk - c.p0) * c.G >> (THIN ? 4 : 7));
-}
-template <bool THIN>
-__device__ __forceinline__ long long pieces_before(const Cut &c, int t) {
-    long long n = (long long)c.c0 * t;
-    for (int i = c.c0; i < c.nc; ++i) n += max(0, t - first_with<THIN>(c, i));
-    return n;
-}
-// Tile t's pieces: n, of len positions each but the last, which may be shorter or, where the tile's positions are fewer
-// than S(t), empty. Thin tiles' are equal up to whole tiles of 128 (what they take is memory, shared evenly); wide
-// tiles' are whole chunks and a rest.
-struct Pieces {
-    int n, len;
-};
-template <bool THIN>
-__device__ __forceinline__ Pieces pieces_of(const Cut &c, int t) {
-    const uint32_t rows = min((uint32_t)(t + 1) * kTileRows<THIN>, (uint32_t)c.rows);
-    const uint32_t span = (uint32_t)max(0, min(c.p0 + (int)((rows + (uint32_t)c.G - 1) / (uint32_t)c.G), c.limit));
-    const uint32_t n = max(1u, (span + (uint32_t)(c.chunk - 1)) / (uint32_t)c.chunk);
-    return {(int)n, THIN ? (int)(((span + n - 1) / n + 127) / 128 * 128) : c.chunk};
-}
-// Item `local` of a head's: its tile and piece, the largest first, so that a queue ends with its smallest. Wide tiles'
-// whole chunks, then the rests: tile t of those with c + 1 pieces has about t - T(c) tiles' rows of positions in its
-// rest, so that the rests in descending order are those of the tiles with t - T(c) >= v for falling v.
-struct TilePiece {
-    int tile, piece;
-};
-template <bool THIN>
-__device__ __forceinline__ TilePiece tile_piece(const Cut &c, int local) {
-    for (int i = c.nc - 1; i >= (THIN ? c.c0 : 1); --i) {
-        const int n = c.nt - (i >= c.c0 ? first_with<THIN>(c, i) : 0);
-        if (local < n) return {c.nt - 1 - local, THIN ? i : i - 1};
-        local -= n;
-    }
-    if (THIN) return {c.nt - 1 - local % c.nt, c.c0 - 1 - local / c.nt};
-    if (c.nc == c.c0) return {c.nt - 1 - local, c.nc - 1};
-    // the tiles of class i (i + 1 pieces) are [from(i), to(i)): how many have t - T(i) >= v
-    auto from = [&](int i) { return i >= c.c0 ? first_with<THIN>(c, i) : 0; };
-    auto to = [&](int i) { return i + 1 < c.nc ? first_with<THIN>(c, i + 1) : c.nt; };
-    auto count = [&](int v) {
-        int n = 0;
-        for (int i = c.c0 - 1; i < c.nc; ++i) n += max(0, to(i) - max(from(i), first_with<THIN>(c, i) + v));
-        return n;
-    };
-    int lo = 0, hi = c.nt - first_with<THIN>(c, c.c0 - 1);  // count(lo) > local >= count(hi)
-    while (hi - lo > 1) {
-        const int mid = (int)(((uint32_t)lo + (uint32_t)hi) >> 1);
-        if (count(mid) > local)
-            lo = mid;
-        else
-            hi = mid;
-    }
-    local -= count(hi);
-    int i = c.c0 - 1;  // of the classes that have a tile at lo
-    for (;; ++i) {
-        const int t = first_with<THIN>(c, i) + lo;
-        if (t >= from(i) && t < to(i) && local-- == 0) break;
-        if (i + 1 == c.nc) break;
-    }
-    return {first_with<THIN>(c, i) + lo, i};
+    int rows = q.m * (int)a.group.d;
+    if (THIN != (a.thin && rows <= kThinRows)) rows = 0;
+    return cut_rows<THIN>(rows, q.n, q.p0, (int)a.group.d, a.window, chunk);
 }
 
 // Rows that a block of attn_merge_kernel joins: a few per wave, or where many pieces have to be read, as many as one
@@ -675,10 +588,10 @@ __device__ int schedule(const AttnArgs &a, int block, int blocks, int32_t *s_ite
             const Request q = req(r);
             if (!q.m) continue;
             const Cut c = cut_of<THIN>(a, q, chunk);
-            const long long n = pieces_before<THIN>(c, c.nt) * a.d.n_kv;
-            v[0] += (int)min(n, 1ll << 30);
+            const int64_t n = pieces_before<THIN>(c, c.nt) * a.d.n_kv;
+            v[0] += (int)min(n, (int64_t)1 << 30);
             if (c.nc > 1) {
-                v[1] = (int)min(v[1] + n * (tr / 16), 1ll << 22);  // more than ever fit, and no sum of them wraps
+                v[1] = (int)min(v[1] + n * (tr / 16), (int64_t)1 << 22);  // more than ever fit, and no sum of them wraps
                 v[2] += (c.rows * a.d.n_kv + merge_rows<HDP>(c.nc) - 1) / merge_rows<HDP>(c.nc);
             }
         }

@@ -517,6 +517,27 @@ def test_attention_of_lengths_out_of_range(dev, up, shape):
     assert np.abs(got[3:8] - ref).max() <= tol
 
 
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_attention_of_more_rows_than_positions(dev, up, dt):
+    """kv_len far below the new rows of a request whose positions are cut: the rows before position 0 are 0, the others
+    see what there is."""
+    s = Step(up, [(0, 3400), (50, 1)], 2, 2, 64, 16, dt, seed=36).upload()
+    n = 3000
+    dev.h2d(s.d_n, np.array([n, 51], np.int32))
+    got = s.run(dev)[:, :s.qd]
+    assert (got[:3400 - n] == 0).all()
+    want = Step(up, [(0, n), (50, 1)], 2, 2, 64, 16, dt, seed=36)
+    want.q = s.q[3400 - n:]
+    want.k, want.v = [s.k[0][:n], s.k[1]], [s.v[0][:n], s.v[1]]
+    ref, tol = want.reference()
+    assert np.abs(got[3400 - n:] - ref).max() <= tol
+
+
+@pytest.mark.parametrize("shape", [(200, 1, 64, 16, BF16), (300, 2, 128, 16, F32)], ids=["200", "150"])
+def test_attention_of_more_heads_than_a_tile(dev, up, shape):
+    Step(up, [(700, 3), (0, 5), (90, 1)], *shape, seed=37).upload().check(dev)
+
+
 def test_attention_of_rows_out_of_order_stays_in_bounds(dev, up):
     """Row starts that do not ascend or pass the rows: some rows are computed, none outside the buffers."""
     s = Step(up, [(30, 8), (10, 3), (20, 2)], 2, 2, 128, 16, BF16, seed=9, spare_rows=2).upload()

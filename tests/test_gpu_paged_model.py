@@ -161,7 +161,8 @@ def test_refusals_of_the_state(dev):
         dev.forward_paged([1], [0], cfg.vocab, cfg.n_layers, cfg.top_k)
     good = dict(n_req=2, ctx=8, n_blocks=4, block_size=4, dtype=F32, max_tokens=4)
     for over in (dict(n_req=0), dict(n_req=4097), dict(ctx=-1), dict(n_blocks=0), dict(block_size=0), dict(dtype=2),
-                 dict(max_tokens=0), dict(max_tokens=65536), dict(n_blocks=1 << 20, block_size=1 << 12)):
+                 dict(max_tokens=0), dict(max_tokens=65536), dict(n_blocks=1 << 20, block_size=1 << 12),
+                 dict(n_blocks=1, block_size=2**31 - 1)):
         with pytest.raises(hip.HipError, match="paged_init"):
             dev.paged_init(**dict(good, **over))
     dev.paged_init(**good)

@@ -129,9 +129,37 @@ def test_null_descriptors():
 INDEX_DRIVER = r"""
 #include <stdio.h>
 #include <initializer_list>
+#include <vector>
 #include "paged.h"
 using namespace rbt;
 #define CHECK(c) do { if (!(c)) { printf("line %d: %s\n", __LINE__, #c); return 1; } } while (0)
+template <bool THIN>
+int check_cut(int n, int m, int G, int window, int chunk) {
+    const int p0 = n - m, tr = kTileRows<THIN>;
+    const Cut c = cut_rows<THIN>(m * G, n, p0, G, window, chunk);
+    CHECK(c.nt == (m * G + tr - 1) / tr);
+    std::vector<std::vector<int>> seen((size_t)c.nt);
+    int64_t all = 0;
+    for (int t = 0; t < c.nt; ++t) {
+        CHECK(pieces_before<THIN>(c, t) == all);
+        const Pieces p = pieces_of<THIN>(c, t);
+        CHECK(p.n >= 1 && p.len >= 0 && p.len <= chunk && (p.len % 128 == 0 || p.len == chunk));
+        // the tile's positions, as its block has them
+        const int64_t r1 = (int64_t)(t + 1) * tr < c.rows ? (int64_t)(t + 1) * tr : c.rows;
+        const int64_t pa = p0 + (int64_t)t * tr / G, pb = p0 + (r1 - 1) / G;
+        const int64_t lo = window > 0 && pa - window + 1 > 0 ? pa - window + 1 : 0, end = pb + 1 > lo ? pb + 1 : lo;
+        CHECK((int64_t)p.n * p.len >= end - lo);
+        seen[(size_t)t].assign((size_t)p.n, 0);
+        all += p.n;
+    }
+    CHECK(pieces_before<THIN>(c, c.nt) == all);
+    for (int64_t i = 0; i < all; ++i) {
+        const TilePiece x = tile_piece<THIN>(c, (int)i);
+        CHECK(x.tile >= 0 && x.tile < c.nt && x.piece >= 0 && x.piece < (int)seen[(size_t)x.tile].size());
+        CHECK(seen[(size_t)x.tile][(size_t)x.piece]++ == 0);
+    }
+    return 0;
+}
 int main() {
     // page_of is the quotient, at the borders of every divisor's multiples and of the range
     for (long long d = 1; d <= 2147483647ll; d = d < 70000 ? d + 1 : d * 3 / 2 + 1) {
@@ -149,6 +177,21 @@ int main() {
     for (int t = 0; t < 9; ++t) CHECK(request_of(start, 8, t) == of[t]);
     const int32_t odd[] = {5, 1, 7, -3, 2};  // rows that do not ascend: in bounds all the same
     for (int t = -10; t < 20; ++t) { const int r = request_of(odd, 4, t); CHECK(r >= 0 && r < 4); }
+    // the cut of a request: every (tile, piece) is one item, and the pieces cover the tile's positions
+    const int ns[] = {0, 1, 5, 100, 128, 129, 700, 1000, 3001}, ms[] = {1, 2, 16, 17, 128, 300, 1500},
+              gs[] = {1, 2, 3, 7, 16, 40, 200}, ws[] = {0, 1, 100, 129, 1000, 2147483647}, cs[] = {128, 256, 640, 1408, kMaxChunk};
+    for (int n : ns) for (int m : ms) for (int g : gs) for (int w : ws) for (int ch : cs) {
+        if ((long long)m * g > 70000) continue;
+        if (check_cut<false>(n, m, g, w, ch) || (m * g <= kThinRows && check_cut<true>(n, m, g, w, ch))) {
+            printf("n %d m %d G %d window %d chunk %d\n", n, m, g, w, ch);
+            return 1;
+        }
+    }
+    // positions and chunks near 2^31
+    for (int ch : {1 << 20, 1 << 30, kMaxChunk - 128})
+        for (int g : {1, 3, 16, 8192})
+            for (int m : {1, 5})
+                if (check_cut<false>(kMaxChunk - 3, m, g, 0, ch) || (m * g <= kThinRows && check_cut<true>(kMaxChunk - 3, m, g, 0, ch))) return 1;
     // offsets past 32 bits
     PagedDims d{1 << 20, 128, 8, 128, 8ull * 128 * 128, page_div(128)};
     CHECK(paged_row(d, (1 << 20) - 1, 7, 127) + 128 == (uint64_t)(1 << 20) * 8 * 128 * 128);
