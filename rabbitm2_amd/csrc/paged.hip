@@ -540,10 +540,11 @@ template <int HDP>
 __device__ __forceinline__ int merge_rows(int nc) { return 256 / HDP * (nc >= kMergeManyPieces ? 1 : 4); }
 
 // A kind's items (request, head, row tile, piece), by every block for itself: prefix sums over the requests into
-// s_items [n_req + 1] and s_units. The chunk length: thin, what spreads the positions over two rounds of blocks, evenly;
-// wide, over one, whose gaps the rests of the tiles fill: fewer partials, fewer diagonals (13 prompts and chunks of 200
-// to 4096 tokens: 127 us on average against 132 with chunks of half that; a windowed prompt of 2 x 2048 67 against
-// 108, three prompts of 1500 169 against 141). It doubles until the partials fit, which ends at the latest at kMaxChunk,
+// s_items [n_req + 1] and s_units. The chunk length is a little over a block's share of
+// the positions, so that most blocks get one piece and the rests fill the gaps: 19 decoding, chunked and prompt steps
+// take 82.6 us on average, 85.0 with half of it for thin tiles (131072 positions 92 against 99, 64 long sequences 218
+// against 217), 89 with half of it for all (a windowed prompt of 2 x 2048 68 against 108, three prompts of 1500 164
+// against 141). It doubles until the partials fit, which ends at the latest at kMaxChunk,
 // where no tile is cut. Returns 0 where no request is of this kind.
 struct ScheduleShared {
     float work[4];
@@ -579,9 +580,8 @@ __device__ int schedule(const AttnArgs &a, int block, int blocks, int32_t *s_ite
         if (hdr && threadIdx.x == 0) hdr->merge_blocks = 0;
         return 0;
     }
-    work = ((s.work[0] + s.work[1]) + (s.work[2] + s.work[3])) * (float)a.d.n_kv / (float)(2 * blocks);
-    int chunk = THIN ? (int)fminf(work, 1.0e9f) / 128 * 128 + 128 : (int)fminf(2 * work + 127, 1.0e9f) / 128 * 128;
-    chunk = max(chunk, 128);
+    work = ((s.work[0] + s.work[1]) + (s.work[2] + s.work[3])) * (float)a.d.n_kv / (float)blocks;
+    int chunk = max((int)fminf(1.025f * work, 1.0e9f), 0) / 128 * 128 + 128;
     for (;;) {
         int v[3] = {0, 0, 0}, inc[3], before[3], total[3];  // items, partial units, merge blocks
         for (int r = r0; r < r1; ++r) {
