@@ -540,12 +540,12 @@ template <int HDP>
 __device__ __forceinline__ int merge_rows(int nc) { return 256 / HDP * (nc >= kMergeManyPieces ? 1 : 4); }
 
 // A kind's items (request, head, row tile, piece), by every block for itself: prefix sums over the requests into
-// s_items [n_req + 1] and s_units. The chunk length is a little over a block's share of
-// the positions, so that most blocks get one piece and the rests fill the gaps: 19 decoding, chunked and prompt steps
-// take 82.6 us on average, 85.0 with half of it for thin tiles (131072 positions 92 against 99, 64 long sequences 218
-// against 217), 89 with half of it for all (a windowed prompt of 2 x 2048 68 against 108, three prompts of 1500 164
-// against 141). It doubles until the partials fit, which ends at the latest at kMaxChunk,
-// where no tile is cut. Returns 0 where no request is of this kind.
+// s_items [n_req + 1] and s_units. The chunk length is a little over a block's share of the positions, so that most
+// blocks get one piece and the rests fill the gaps: 19 decoding, chunked and prompt steps take 82.6 us on average, and
+// 85.0 with half of it for thin tiles (131072 positions 92 against 99 us, 64 long sequences 218 against 217); half of it
+// for wide tiles: a windowed prompt of 2 x 2048 tokens 108 against 68, three prompts of 1500 141 against 164. It doubles
+// until the partials fit, which ends at the latest at kMaxChunk, where no tile is cut. Returns 0 where no request is of
+// this kind.
 struct ScheduleShared {
     float work[4];
     int any[4], sum[4][3];
@@ -1080,18 +1080,21 @@ __device__ __forceinline__ Item item_of(const AttnArgs &a, int it, int chunk, co
               ((size_t)x.kvh * pieces + (size_t)pieces_before<THIN>(x.cut, tile) + c) * (tr / 16)) * unit_floats(HDP);
     return x;
 }
-// An eighth of the items to each XCD (blocks b % 8), so that a head's row tiles read its keys and values through one
-// L2. A block starts with the item of its own number and, where there are more items than blocks, then takes the next
+// An eighth of the items to each XCD (blocks b % 8): with a multiple of eight heads, or an item per block at most, a run
+// of them, so that a head's row tiles read its keys and values through one L2; otherwise every eighth item, so that each
+// XCD gets large and small ones (prompt of 2048, 8 heads of 256 on 2: 175 us, 255 by runs; 2000 positions, 16 on 4: 77
+// and 88; three chunks of 333, 16 heads of 64 on 4: 43.7 and 40.6). A block starts with the item of its own number and, where there are more items than blocks, then takes the next
 // one left of its eighth, then of the other eighths: ask() early, its answer used by next() at the item's end.
 struct ItemQueue {
     int it, n, xcd, per;  // it < 0: nothing is left
-    bool more;
+    bool runs, more;
     AttnHeader *hdr;
     __device__ __forceinline__ int start(int x) const { return (int)((long long)n * x / 8); }
-    __device__ __forceinline__ ItemQueue(int n_items, AttnHeader *header, int block, int blocks)
-        : n(n_items), xcd(block & 7), per(blocks >> 3), more(n_items > blocks), hdr(header) {
-        it = start(xcd) + (block >> 3);
-        if (it >= start(xcd + 1)) it = -1;
+    __device__ __forceinline__ int count(int x) const { return runs ? start(x + 1) - start(x) : (n - x + 7) >> 3; }
+    __device__ __forceinline__ int item(int x, int k) const { return runs ? start(x) + k : x + 8 * k; }
+    __device__ __forceinline__ ItemQueue(int n_items, int n_kv, AttnHeader *header, int block, int blocks)
+        : n(n_items), xcd(block & 7), per(blocks >> 3), runs(n_kv % 8 == 0 || n_items <= blocks), more(n_items > blocks), hdr(header) {
+        it = (block >> 3) < count(xcd) ? item(xcd, block >> 3) : -1;
     }
     __device__ __forceinline__ int ask() const { return more && threadIdx.x == 0 ? atomicAdd(&hdr->taken[xcd][0], 1) : 0; }
     // for all threads
@@ -1100,10 +1103,11 @@ struct ItemQueue {
         while (more) {
             if (threadIdx.x < kWave) {  // the answer, or the first other eighth with any left (its counters only grow)
                 const int x = threadIdx.x & 7;
-                int got = __builtin_amdgcn_readfirstlane(ticket) + start(xcd) + per;
-                if (got >= start(xcd + 1)) {
+                const int k = __builtin_amdgcn_readfirstlane(ticket) + per;
+                int got = item(xcd, k);
+                if (k >= count(xcd)) {
                     const int t = __hip_atomic_load(&hdr->taken[x][0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                    const uint32_t left = (uint32_t)__ballot(start(x) + per + t < start(x + 1)) & 0xFFu;
+                    const uint32_t left = (uint32_t)__ballot(per + t < count(x)) & 0xFFu;
                     got = left ? -2 - (__ffs((int)left) - 1) : -1;
                 }
                 if (threadIdx.x == 0) *s_next = got;
@@ -1274,7 +1278,7 @@ __device__ __forceinline__ void attn_thin(const AttnArgs &a, int block, int bloc
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
     const int chunk = __builtin_amdgcn_readfirstlane(schedule<true, HDP>(a, block, blocks, s_items, s_units, s_sched));
     if (chunk == 0) return;
-    ItemQueue items(__builtin_amdgcn_readfirstlane(s_items[a.n_req]), AttnWs<true>::header(a.ws), block, blocks);
+    ItemQueue items(__builtin_amdgcn_readfirstlane(s_items[a.n_req]), a.d.n_kv, AttnWs<true>::header(a.ws), block, blocks);
     const int span = tab_span(a);
     const PaddedTile<HDP> tl;
     while (items.it >= 0) {
@@ -1424,7 +1428,7 @@ __device__ __forceinline__ void attn_wide(const AttnArgs &a, int block, int bloc
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
     const int chunk = __builtin_amdgcn_readfirstlane(schedule<false, HDP>(a, block, blocks, s_items, s_units, s_sched));
     if (chunk == 0) return;
-    ItemQueue items(__builtin_amdgcn_readfirstlane(s_items[a.n_req]), AttnWs<false>::header(a.ws), block, blocks);
+    ItemQueue items(__builtin_amdgcn_readfirstlane(s_items[a.n_req]), a.d.n_kv, AttnWs<false>::header(a.ws), block, blocks);
     const int span = tab_span(a);
     const typename Sh::Tile tl;
     while (items.it >= 0) {
