@@ -500,7 +500,7 @@ __global__ __launch_bounds__(256) void attn_any_kernel(AttnArgs a) {
 //
 // What bounds it: a prompt of 4096 tokens (16 heads of 128, bf16) takes 208 us, 206 GFLOP in its three products: 990
 // TFLOP/s, where a large library product reaches 1200; the matrix units are busy 75% of the inner loop, items' starts
-// and ends and the joining of pieces take 20 us each. 64 decoding sequences of up to 8192 positions take 216 us, 5.8
+// and ends and the joining of pieces take 20 us each. 64 decoding sequences of up to 8192 positions take 218 us, 5.7
 // TB/s of cache. Small steps are latency: the schedule, pages, queries and first keys one after the other, and two
 // launches (one sequence: 16 us).
 //
