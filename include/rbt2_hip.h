@@ -298,7 +298,7 @@ typedef struct {
 /* The requests of a step: request r has kv_len[r] positions in the cache, this step's among them; position p
  * is row p % block_size of block tables[r * max_blocks + p / block_size]. Rows q_start[r] .. q_start[r + 1] - 1
  * of the step's row buffers are its new tokens, the last positions of the request. n_req up to 4096. A request
- * without new rows takes no part. */
+ * without new rows, or whose rows do not lie within the buffers', takes no part. */
 typedef struct {
     int32_t n_req, max_blocks;
     const int32_t *tables;  /* [n_req][max_blocks] */
